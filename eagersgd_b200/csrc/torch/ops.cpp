@@ -1534,6 +1534,10 @@ Tensor lstm_layer(const Tensor& x, const Tensor& w_ih, const Tensor& w_hh, const
 
 }  // namespace
 
+#include "group_norm.h"
+#include "distill.h"
+#include "scan.h"
+
 PYBIND11_MODULE(_esgd_torch, m) {
   m.doc() = "autograd operators over the sm_100a kernels of eagersgd_b200";
   m.def("error_flag", &error_flag);
@@ -1553,6 +1557,12 @@ PYBIND11_MODULE(_esgd_torch, m) {
   m.def("residual_block_eval", &residual_block_eval);
   m.def("softmax_ce", &softmax_ce);
   m.def("lstm_layer", &lstm_layer);
+  m.def("group_norm_act", &group_norm_act);
+  m.def("distillation_loss", &distillation_loss);
+  m.def("causal_conv", &causal_conv);
+  m.def("causal_conv_step", &causal_conv_step);
+  m.def("selective_scan", &selective_scan);
+  m.def("selective_scan_step", &selective_scan_step);
   m.def("max_pool", &max_pool);
   m.def("avg_pool", &avg_pool);
   py::class_<ZeroArena, std::shared_ptr<ZeroArena>>(m, "ZeroArena")

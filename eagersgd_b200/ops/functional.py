@@ -160,6 +160,39 @@ def residual_block(x: torch.Tensor, layers, proj=None) -> Optional[torch.Tensor]
     return _ext().residual_block(x, layers, proj, _SMALL_CHANNELS_NATIVE) if native(x) else None
 
 
+# --------------------------------------------------------------------------- group norm (+ residual) (+ activation)
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2}
+
+
+def activation_code(op: str, activation: Optional[str], taken=(None, "relu", "silu")) -> int:
+    if activation not in taken:
+        raise ValueError("%s: the activation %r is none of %s" % (op, activation, ", ".join(map(repr, taken))))
+    return _ACTIVATIONS[activation]
+
+
+def native_float(x: torch.Tensor) -> bool:
+    """Whether the kernels that take bf16 and fp32 take ``x``."""
+    return x.is_cuda and x.dtype in (torch.bfloat16, torch.float32) and not _reference_only
+
+
+def group_norm_act(x: torch.Tensor, groups: int, gamma: torch.Tensor, beta: torch.Tensor, activation: Optional[str] = None,
+                   residual: Optional[torch.Tensor] = None, eps: float = BN_EPS) -> torch.Tensor:
+    """z = act(gamma * (x - mean) / sqrt(var + eps) + beta [+ residual]) with the statistics of a sample's group of channels.
+
+    ``x`` [N, C, H, W] bf16 or fp32, ``gamma`` and ``beta`` fp32 [C], ``activation`` None, "relu" or "silu".  Unlike
+    ``bn_act`` it keeps no statistics and does the same in training and inference: what a replica computes does not depend on
+    which samples the others have.  Up to 4096 channels a group."""
+    act = activation_code("group_norm_act", activation)
+    if native_float(x):
+        return _ext().group_norm_act(x, groups, gamma, beta, act, residual, eps)
+    wide = x if x.dtype in (torch.float32, torch.float64) else x.float()
+    z = F.group_norm(wide, groups, gamma.to(wide.dtype), beta.to(wide.dtype), eps)
+    if residual is not None:
+        z = z + residual.to(wide.dtype)
+    z = F.relu(z) if activation == "relu" else F.silu(z) if activation == "silu" else z
+    return z.to(x.dtype)
+
+
 # --------------------------------------------------------------------------- inference: convolution + batch norm in one kernel
 def bn_coefficients(layers, store):
     """Scale and shift (``[2 * C]`` fp32, one after the other) of each inference batch norm in ``layers`` -- tuples of gamma,
@@ -202,6 +235,36 @@ def softmax_cross_entropy(logits: torch.Tensor, labels: torch.Tensor) -> torch.T
             and not _reference_only:
         return _ext().softmax_ce(logits, labels)
     return F.cross_entropy(logits.float(), labels)
+
+
+def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_classes: torch.Tensor, temperature: float = 1.0,
+                      labels: Optional[torch.Tensor] = None, hard_weight: float = 0.0) -> torch.Tensor:
+    """Mean over the rows of ``(1 - hard_weight) * T^2 * KL(p || softmax(logits / T)) + hard_weight * cross_entropy(logits, labels)``
+    where ``p = softmax(teacher_logits / T)`` over the classes that the teacher names.
+
+    ``logits`` [rows, classes] and ``teacher_logits`` [rows, top] are bf16 or fp32 (each on its own), ``teacher_classes``
+    [rows, top] and ``labels`` [rows] int64; ``top`` up to 1024.  An index outside the classes (-1 where a teacher names fewer) and a
+    teacher's logit of -inf are left out, a class that is named twice counts twice, and a row without a teacher or label has no such
+    term.  The gradient goes to ``logits`` alone; it is made with the loss, in one pass over the logits, and rounded to their type."""
+    if native_float(logits):
+        return _ext().distillation_loss(logits, teacher_logits, teacher_classes, temperature, labels, hard_weight)
+    if labels is None and hard_weight != 0:
+        raise ValueError("distillation_loss: a hard weight without labels")
+    wide = logits if logits.dtype == torch.float64 else logits.float()
+    classes, t = logits.shape[1], temperature
+    named = (teacher_classes >= 0) & (teacher_classes < classes) & (teacher_logits != -float("inf"))
+    values = torch.where(named, teacher_logits.detach().to(wide.dtype) / t, -float("inf"))
+    taught = named.any(1, keepdim=True)
+    log_p = torch.log_softmax(torch.where(taught, values, 0.0), 1)
+    log_q = torch.log_softmax(wide / t, 1).gather(1, teacher_classes.clamp(0, classes - 1))
+    p = torch.where(named, log_p.exp(), 0.0)
+    kl = torch.where(p > 0, p * (torch.where(p > 0, log_p, 0.0) - torch.where(p > 0, log_q, 0.0)), 0.0).sum(1)
+    loss = (1.0 - hard_weight) * t * t * kl.sum() / logits.shape[0]
+    if hard_weight != 0:
+        valid = (labels >= 0) & (labels < classes)
+        ce = F.cross_entropy(wide, torch.where(valid, labels, 0), reduction="none")
+        loss = loss + hard_weight * torch.where(valid, ce, 0.0).sum() / logits.shape[0]
+    return loss
 
 
 # --------------------------------------------------------------------------- pooling
