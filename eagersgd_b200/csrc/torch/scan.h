@@ -12,11 +12,13 @@ int esgd_causal_conv_bwd(const void* x, int64_t xb, int64_t xt, const void* stat
                          int64_t length, int channels, int taps, int act, void* stream);
 int esgd_causal_conv_step(const void* x, int64_t xb, const void* state, void* state_out, const float* weight, const float* bias, void* y,
                           int is_bf16, int64_t batch, int channels, int taps, int act, void* stream);
-int64_t esgd_selective_scan_keep(int64_t batch, int64_t length, int channels, int states);
-int64_t esgd_selective_scan_narrow(int64_t batch, int64_t length, int channels, int states);
-int esgd_selective_scan_fwd(const esgd_scan* e, void* out, float* state_out, float* keep, void* stream);
+int64_t esgd_selective_scan_local(const esgd_scan* e);
+int64_t esgd_selective_scan_keep(const esgd_scan* e);
+int64_t esgd_selective_scan_narrow(const esgd_scan* e);
+int64_t esgd_selective_scan_parts(const esgd_scan* e);
+int esgd_selective_scan_fwd(const esgd_scan* e, void* out, float* state_out, float* keep, float* local, void* stream);
 int esgd_selective_scan_bwd(const esgd_scan* e, const void* dout, const float* keep, void* du, void* ddelta, void* dz, void* dB, void* dC,
-                            float* narrow, float* sums, void* stream);
+                            float* narrow, float* sums, float* local, void* stream);
 int esgd_selective_scan_step(const esgd_scan* e, float* state_out, void* out, void* stream);
 }
 
@@ -49,6 +51,7 @@ Tensor state_for(const char* op, const Opt& out, const Tensor& state) {
   TORCH_CHECK(a == b || a + state.nbytes() <= b || b + out->nbytes() <= a, op, ": out overlaps the state without being it");
   return *out;
 }
+Tensor room(int64_t floats, const at::TensorOptions& f32) { return floats > 0 ? at::empty({floats}, f32) : Tensor(); }
 void written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 
 // ---------------------------------------------------------------- causal convolution
@@ -214,9 +217,10 @@ struct SelectiveScanFn : public Function<SelectiveScanFn> {
     const esgd_scan e = in.args();
     variable_list out = {at::empty(in.u.sizes(), in.u.options())};
     if (want_state) out.push_back(at::empty({e.batch, e.channels, e.states}, in.A.options()));
-    if (keep != nullptr) *keep = at::empty({esgd_selective_scan_keep(e.batch, e.length, e.channels, e.states)}, in.A.options());
-    ck(esgd_selective_scan_fwd(&e, mut(out[0]), want_state ? fptr(out[1]) : nullptr, keep != nullptr ? fptr(*keep) : nullptr, stream_of(in.u)),
-       "selective_scan");
+    if (keep != nullptr) *keep = at::empty({esgd_selective_scan_keep(&e)}, in.A.options());
+    const Tensor local = room(esgd_selective_scan_local(&e), in.A.options());
+    ck(esgd_selective_scan_fwd(&e, mut(out[0]), want_state ? fptr(out[1]) : nullptr, keep != nullptr ? fptr(*keep) : nullptr, fptr(local),
+                               stream_of(in.u)), "selective_scan");
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -235,11 +239,11 @@ struct SelectiveScanFn : public Function<SelectiveScanFn> {
     Tensor du = at::empty(in.u.sizes(), in.u.options()), ddelta = at::empty_like(du), dz = in.z.defined() ? at::empty_like(du) : Tensor();
     Tensor dB = at::empty({e.batch, e.length, n}, in.u.options()), dC = at::empty_like(dB);
     const ParamGrad dA(ctx, "A", need[0], {d, n}, f32), dD(ctx, "D", need[1], {d}, f32), db(ctx, "b", need[2], {d}, f32);
-    const int64_t parts = e.length > 0 ? e.batch : 0;
-    Tensor narrow = at::empty({esgd_selective_scan_narrow(e.batch, e.length, e.channels, e.states)}, f32);
-    Tensor sums = at::empty({parts, d * (n + 2)}, f32);
+    const int64_t parts = esgd_selective_scan_parts(&e);
+    const Tensor narrow = at::empty({esgd_selective_scan_narrow(&e)}, f32), sums = at::empty({parts, d * (n + 2)}, f32);
+    const Tensor local = room(esgd_selective_scan_local(&e), f32);
     ck(esgd_selective_scan_bwd(&e, ptr(dout), fptr(keep), mut(du), mut(ddelta), mut(dz), mut(dB), mut(dC), fptr(narrow), fptr(sums),
-                               stream_of(in.u)), "selective_scan backward");
+                               fptr(local), stream_of(in.u)), "selective_scan backward");
     ck(esgd_sum_parts(fptr(sums), parts, dA.out(), d * n, dA.add(), dD.out(), d, dD.add(), db.out(), d, db.add(), stream_of(in.u)),
        "selective_scan parameter gradients");
     dA.done();

@@ -206,8 +206,8 @@ def _scan_check(c, dy, softplus=True, state=None, lengths=None):
     big = lambda v: v.max().item() if v.numel() else 0.0  # noqa: E731
     for k, got, wanted in zip(names, gots, wants):
         if k in ("B", "C"):
-            # sums over the channels of products of a state: in bf16 the products' factors may have bf16's next eleven bits only
-            bits = 2.0 ** 13 if c["u"].dtype == BF16 else 0.0
+            # sums over the channels of products of a state: with bf16 sequences the two factors have eleven bits, each off by half a step
+            bits = 2.0 ** 14 if c["u"].dtype == BF16 else 0.0
             near(got, wanted, big(amp[k]), 2 * steps + bits, "d" + k)
         elif k in ("delta", "delta_bias"):
             near(got, wanted, big(amp["dt"]) if k == "delta" else amp["dt"].sum((0, 1)).max().item(), 4 * steps, "d" + k)
