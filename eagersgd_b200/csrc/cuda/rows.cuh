@@ -61,13 +61,19 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // e^x with the rounding of x * log2(e) put right to first order: without it the relative error grows with |x| (20: 2e-6).
 __device__ __forceinline__ float exp_fine(float x) {
   const float t = x * kLog2e, y = exp2_approx(t);
   const float low = fmaf(x, kLog2eLow, fmaf(x, kLog2e, -t));
   return fabsf(t) < 128.0f ? fmaf(y, low * kLn2, y) : y;      // beyond it y is 0 or infinite (or t is, and low no number)
 }
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + exp_fine(-x)); }
+// For the gates: where the exponential's error grows, far below zero, the result is next to nothing; above zero it is next to one.
+__device__ __forceinline__ float sigmoid(float x) { return reciprocal(1.0f + exp2_approx(x * -kLog2e)); }
 
 // An activation and its slope at x.
 template <int kAct> __device__ __forceinline__ float activate(float x) {

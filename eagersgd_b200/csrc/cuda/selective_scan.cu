@@ -59,7 +59,18 @@ __device__ __forceinline__ int64_t length_of(const Scan& s, int64_t b) {
   const int64_t n = s.lengths[b];
   return n < 0 ? 0 : n > s.length ? s.length : n;
 }
-__device__ __forceinline__ float softplus(float x) { return x > 20.0f ? x : log1pf(exp_fine(x)); }
+
+// log(1 + e^x) = max(x, 0) + log(1 + v) with v = e^-|x|, and log(1 + v) = 2 artanh(v / (2 + v)): an odd function whose argument
+// is at most 1/3, so five terms, fitted to the relative error, are right to 4e-9.  slope: 1 / (1 + e^-x).
+__device__ __forceinline__ float softplus(float x, float* slope = nullptr) {
+  const float v = exp2_approx(fminf(fabsf(x), 120.0f) * -kLog2e);
+  const float r = v * reciprocal(2.0f + v), q = r * r;
+  const float log = fmaf(fmaf(fmaf(fmaf(0.281614542f, q, 0.279643446f), q, 0.400246501f), q, 0.666663229f), q, 2.0f);
+  float top;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(x), "f"(0.0f));
+  if (slope != nullptr) *slope = reciprocal(1.0f + v) * (x < 0.0f ? v : 1.0f);
+  return fmaf(r, log, top);
+}
 
 // Two neighbouring values as they lie in memory.
 template <class T> struct Two;
@@ -154,6 +165,8 @@ template <int kWide_> struct Block {
 template <class T, int kLanes> struct Ahead {
   static constexpr int kWide = kThreads / kLanes, kPadded = kLanes * kStates;
   static constexpr int kPairs = kTile * kWide / 2 <= kThreads ? 1 : kTile * kWide / 2 / kThreads;
+  // a row of partial sums: a warp's channels of every lane fall into banks of their own
+  static constexpr int kRow = kWide + (32 / kLanes - kWide % 32 + 32) % 32;
   static constexpr int kNarrow = kTile * kPadded / 2 <= kThreads ? 1 : kTile * kPadded / 2 / kThreads;
   __device__ static __forceinline__ int step(int k) { return (threadIdx.x + k * kThreads) / (kWide / 2); }
   __device__ static __forceinline__ int channel(int k) { return (threadIdx.x + k * kThreads) % (kWide / 2) * 2; }
@@ -185,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
   extern __shared__ float4 smem4[];
   float4* s_bc = smem4;                                                   // [kTile][kLanes][2]: four of B, four of C
   float4* s_dt = s_bc + kTile * 2 * kLanes;                               // [kTile][kWide]: dt twice, dt * u twice
-  float* s_y = reinterpret_cast<float*>(s_dt + kTile * kWide);            // [kTile][kWide][kLanes]
+  float* s_y = reinterpret_cast<float*>(s_dt + kTile * kWide);            // [kTile][kLanes][In::kRow]
   const Block<kWide> p(s);
   const int c = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, channel = p.c0 + c;
   const bool on = channel < s.channels;
@@ -271,16 +284,20 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
       const ulonglong2 dt = dt2[t * kWide], b2 = bc2[t * 2 * kLanes], c2 = bc2[t * 2 * kLanes + 1];
       h0 = fma2(exp2_2(mul2(dt.x, a0)), h0, mul2(dt.y, b2.x));
       h1 = fma2(exp2_2(mul2(dt.x, a1)), h1, mul2(dt.y, b2.y));
-      s_y[t * kThreads + threadIdx.x] = sum_of(fma2(c2.y, h1, mul2(c2.x, h0)));
+      s_y[(t * kLanes + lane) * In::kRow + c] = sum_of(fma2(c2.y, h1, mul2(c2.x, h0)));
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < In::kPairs; ++k) {
       if (In::step(k) >= steps) continue;
-      const float* from = s_y + (In::step(k) * kWide + In::channel(k)) * kLanes;
+      const float* from = s_y + In::step(k) * kLanes * In::kRow + In::channel(k);
       float v = 0.0f, w = 0.0f;
 #pragma unroll
-      for (int l = 0; l < kLanes; ++l) { v += from[l]; w += from[kLanes + l]; }
+      for (int l = 0; l < kLanes; ++l) {
+        const float2 part = *reinterpret_cast<const float2*>(from + l * In::kRow);
+        v += part.x;
+        w += part.y;
+      }
       put<T>(y + (t0 + In::step(k)) * s.channels, p.c0 + In::channel(k), s.channels, s.channels % 2 == 0, (v + du[k].x) * gate[k].x,
              (w + du[k].y) * gate[k].y);
     }
@@ -444,12 +461,13 @@ template <class T, int kBlocks>
 __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s, Grads g) {
   pdl_enter();
   constexpr int kWarps = kThreads / 32, kWide = 8 * kWarps / kBlocks, kPadded = 16 * kBlocks, kSlots = 8 * kBlocks;
+  constexpr int kRow = kWide + 4;                            // a warp's eight slots of four channels fall into banks of their own
   constexpr bool kFine = sizeof(T) == 4;
   __shared__ float4 s_bc[kKeep][kSlots];                     // B of states n and n + 8, C of them
   __shared__ float4 s_dt[kKeep][kWide];                      // dt twice, dt u twice
   __shared__ __align__(16) float2 s_dy[kKeep][kWide];                      // dy twice
-  __shared__ __align__(16) float s_part[3][kKeep][kWide][kSlots];          // C h, B dh, A a h[t - 1] dh of a thread's two states
-  __shared__ float s_narrow[kWarps / kBlocks][2][kKeep][kPadded];   // dB, dC over a warp's channels
+  __shared__ __align__(16) float s_part[3][kKeep][kSlots][kRow];           // C h, B dh, A a h[t - 1] dh of a thread's two states
+  __shared__ float s_narrow[kWarps / kBlocks][2][kKeep][kPadded + 4];   // dB, dC over a warp's channels
   const Block<kWide> p(s);
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, part = warp % kBlocks, group = warp / kBlocks;
   const int slot = part * 8 + lane / 4, n0 = part * 16 + lane / 4, w0 = group * 8 + lane % 4;     // state, channel in the block
@@ -522,8 +540,9 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
         const float2 dv = delta.get(), ov = up.get();
         uv = u.get();
         const float x = dv.x + bias.x, w = dv.y + bias.y;
-        dt = s.softplus ? make_float2(softplus(x), softplus(w)) : make_float2(x, w);
-        slope_dt = s.softplus ? make_float2(sigmoid(x), sigmoid(w)) : make_float2(1.0f, 1.0f);
+        dt = make_float2(x, w);
+        slope_dt = make_float2(1.0f, 1.0f);
+        if (s.softplus) dt = make_float2(softplus(x, &slope_dt.x), softplus(w, &slope_dt.y));
         dy = ov;
         if (s.z.p != nullptr) {
           const float2 zv = z.get();
@@ -578,9 +597,9 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
         carry[i] = mul2(a[t][i], dh[i]);
         const f2 da = mul2(carry[i], h[t][i]);
         dA[i] = fma2(da, d.x, dA[i]);
-        s_part[0][t][w0 + 4 * i][slot] = sum_of(mul2(bc.y, h[t + 1][i]));
-        s_part[1][t][w0 + 4 * i][slot] = sum_of(mul2(bc.x, dh[i]));
-        s_part[2][t][w0 + 4 * i][slot] = sum_of(mul2(da, A[i]));
+        s_part[0][t][slot][w0 + 4 * i] = sum_of(mul2(bc.y, h[t + 1][i]));
+        s_part[1][t][slot][w0 + 4 * i] = sum_of(mul2(bc.x, dh[i]));
+        s_part[2][t][slot][w0 + 4 * i] = sum_of(mul2(da, A[i]));
         const bool column = lane / 4 == t;
         by[i] = column ? halves(y2).x : 0.0f;
         bu[i] = column ? halves(d.y).x : 0.0f;
@@ -621,7 +640,11 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
       for (int q = 0; q < 3; ++q) {
         float x = 0.0f, w = 0.0f;
 #pragma unroll
-        for (int l = 0; l < kSlots; ++l) { x += s_part[q][pt][pc][l]; w += s_part[q][pt][pc + 1][l]; }
+        for (int l = 0; l < kSlots; ++l) {
+          const float2 o = *reinterpret_cast<const float2*>(&s_part[q][pt][l][pc]);
+          x += o.x;
+          w += o.y;
+        }
         v[q] = make_float2(x, w);
       }
       const int64_t row = (base + t0 + pt) * s.channels;
@@ -649,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
     for (int j = 0; j < 2; ++j)
       if (ch[i] < s.channels && n0 + 8 * j < s.states) sums[(int64_t)ch[i] * s.states + n0 + 8 * j] = dA_sum[i][j];
   __syncthreads();
-  float4* stage = reinterpret_cast<float4*>(&s_part[0][0][0][0]);      // room for one of each thread: 3 * 8 * 64 float4
+  float4* stage = reinterpret_cast<float4*>(&s_part[0][0][0][0]);      // room for one of each thread
   stage[threadIdx.x] = make_float4(dD.x, dD.y, dbias.x, dbias.y);
   __syncthreads();
   if (threadIdx.x < kPairs) {
@@ -739,7 +762,7 @@ constexpr int64_t kShortest = 128;
 template <class T, int kLanes> int forward(const Scan& s, void* out, float* state_out, float* keep, void* stream) {
   static SmemAllowed allowed{0};
   constexpr int kWide = kThreads / kLanes;
-  constexpr size_t kSmem = kTile * (2 * kLanes * 16 + kWide * 16 + kThreads * 4);
+  constexpr size_t kSmem = kTile * (2 * kLanes * 16 + kWide * 16 + kLanes * Ahead<T, kLanes>::kRow * 4);
   if (kSmem > 48 * 1024) {
     const int rc = allow_smem(selective_scan_fwd_kernel<T, kLanes>, kSmem, allowed);
     if (rc != 0) return rc;
