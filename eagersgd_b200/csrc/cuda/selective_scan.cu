@@ -88,17 +88,8 @@ template <> struct Two<__nv_bfloat16> {
   }
   __device__ __forceinline__ float2 get() const { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 };
-// Values c and c + 1 of a row of `width`, zero beyond it.
-template <class T> __device__ __forceinline__ Two<T> fetch(const T* row, int c, int width, int even) {
-  Two<T> r;
-  if (even && c < width) r.load(row + c);
-  else r.set(c < width ? row[c] : as_type<T>(0.0f), c + 1 < width ? row[c + 1] : as_type<T>(0.0f));
-  return r;
-}
-template <class T> __device__ __forceinline__ Two<T> fetch(const Seq& q, int64_t b, int64_t t, int c, int width, int even) {
-  return fetch<T>(reinterpret_cast<const T*>(q.p) + b * q.b + t * q.t, c, width, even);
-}
-template <class T> __device__ __forceinline__ void put(T* row, int c, int width, int even, float x, float y) {
+// The values c and c + 1 of a row, as far as its width goes.
+template <class T> __device__ __forceinline__ void put(T* row, int c, int width, bool even, float x, float y) {
   if (even && c < width) {
     if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(row + c) = make_float2(x, y);
     else *reinterpret_cast<__nv_bfloat162*>(row + c) = __floats2bfloat162_rn(x, y);
@@ -161,17 +152,49 @@ template <int kWide_> struct Block {
   }
 };
 
-// The steps' operands of a thread, fetched a tile ahead: kPairs pairs of channels and kNarrow pairs of states.
-template <class T, int kLanes> struct Ahead {
-  static constexpr int kWide = kThreads / kLanes, kPadded = kLanes * kStates;
-  static constexpr int kPairs = kTile * kWide / 2 <= kThreads ? 1 : kTile * kWide / 2 / kThreads;
-  // a row of partial sums: a warp's channels of every lane fall into banks of their own
-  static constexpr int kRow = kWide + (32 / kLanes - kWide % 32 + 32) % 32;
-  static constexpr int kNarrow = kTile * kPadded / 2 <= kThreads ? 1 : kTile * kPadded / 2 / kThreads;
-  __device__ static __forceinline__ int step(int k) { return (threadIdx.x + k * kThreads) / (kWide / 2); }
-  __device__ static __forceinline__ int channel(int k) { return (threadIdx.x + k * kThreads) % (kWide / 2) * 2; }
-  __device__ static __forceinline__ int narrow_step(int k) { return (threadIdx.x + k * kThreads) / (kPadded / 2); }
-  __device__ static __forceinline__ int state(int k) { return (threadIdx.x + k * kThreads) % (kPadded / 2) * 2; }
+// What a thread fetches of a tile of kSteps steps: kPairs pairs of channels, always the same two and kPitch steps apart, and kNarrow
+// pairs of states.
+template <int kSteps, int kWide_, int kPadded_> struct Share {
+  static constexpr int kWide = kWide_, kPadded = kPadded_;
+  static constexpr int kPitch = kThreads / (kWide / 2), kPairs = kSteps <= kPitch ? 1 : kSteps / kPitch;
+  static constexpr int kNarrowPitch = kThreads / (kPadded / 2), kNarrow = kSteps <= kNarrowPitch ? 1 : kSteps / kNarrowPitch;
+  int channel, step, state, narrow_step;
+  __device__ Share() {
+    channel = threadIdx.x % (kWide / 2) * 2;
+    step = threadIdx.x / (kWide / 2);
+    state = threadIdx.x % (kPadded / 2) * 2;
+    narrow_step = threadIdx.x / (kPadded / 2);
+  }
+};
+
+// A thread's pairs of one operand: where the next tile's are.
+template <class T> struct Cursor {
+  const T* p;
+  int64_t pitch, tile;       // elements between a thread's pairs, and to the next tile
+  __device__ __forceinline__ void set(const Seq& q, int64_t b, int64_t t, int c, int pitch_, int tile_) {
+    p = reinterpret_cast<const T*>(q.p) + (b * q.b + t * q.t + c);
+    pitch = pitch_ * q.t;
+    tile = tile_ * q.t;
+  }
+  // `n` steps are left from the thread's first on; `in`: how many of the two values there are.
+  template <int kPairs> __device__ __forceinline__ void fetch(Two<T> (&to)[kPairs], int n, int between, int in, bool even) {
+    if (even) {
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k)
+        if (k * between < n && in > 0) to[k].load(p + k * pitch);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k)
+        if (k * between < n) to[k].set(in > 0 ? p[k * pitch] : as_type<T>(0.0f), in > 1 ? p[k * pitch + 1] : as_type<T>(0.0f));
+    }
+    p += tile;
+  }
+};
+__device__ __forceinline__ int left_of(int width, int c) { return width - c < 0 ? 0 : width - c > 2 ? 2 : width - c; }
+
+// Forward passes.  A row of partial sums: a warp's channels of every lane fall into banks of their own.
+template <int kLanes> struct Lanes : Share<kTile, kThreads / kLanes, kLanes * kStates> {
+  static constexpr int kRow = kThreads / kLanes + (32 / kLanes - kThreads / kLanes % 32 + 32) % 32;
 };
 
 // The states that a block begins with: the given one (forward) or none (backward), and the other chunks' joined to it.
@@ -193,15 +216,39 @@ template <class T, int kLanes>
 __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T* __restrict__ out, float* __restrict__ state_out,
                                                                       float* __restrict__ keep) {
   pdl_enter();
-  using In = Ahead<T, kLanes>;
+  using In = Lanes<kLanes>;
   constexpr int kWide = In::kWide, kPadded = In::kPadded;
   extern __shared__ float4 smem4[];
   float4* s_bc = smem4;                                                   // [kTile][kLanes][2]: four of B, four of C
   float4* s_dt = s_bc + kTile * 2 * kLanes;                               // [kTile][kWide]: dt twice, dt * u twice
   float* s_y = reinterpret_cast<float*>(s_dt + kTile * kWide);            // [kTile][kLanes][In::kRow]
   const Block<kWide> p(s);
+  const In in;
   const int c = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, channel = p.c0 + c;
   const bool on = channel < s.channels;
+  const int two = left_of(s.channels, p.c0 + in.channel), narrow_two = left_of(s.states, in.state);
+  Cursor<T> at_u, at_delta, at_z, at_b, at_c;
+  Two<T> u[In::kPairs], delta[In::kPairs], z[In::kPairs], bb[In::kNarrow], cc[In::kNarrow];
+  at_u.set(s.u, p.b, p.first + in.step, p.c0 + in.channel, In::kPitch, kTile);
+  at_delta.set(s.delta, p.b, p.first + in.step, p.c0 + in.channel, In::kPitch, kTile);
+  at_z.set(s.z, p.b, p.first + in.step, p.c0 + in.channel, In::kPitch, kTile);
+  at_b.set(s.B, p.b, p.first + in.narrow_step, in.state, In::kNarrowPitch, kTile);
+  at_c.set(s.C, p.b, p.first + in.narrow_step, in.state, In::kNarrowPitch, kTile);
+  const bool gated = s.z.p != nullptr;
+  auto prefetch = [&](int steps) {
+    const int n = steps - in.step, m = steps - in.narrow_step;
+    at_u.template fetch<In::kPairs>(u, n, In::kPitch, two, s.even);
+    at_delta.template fetch<In::kPairs>(delta, n, In::kPitch, two, s.even);
+    if (gated) at_z.template fetch<In::kPairs>(z, n, In::kPitch, two, s.even);
+    at_b.template fetch<In::kNarrow>(bb, m, In::kNarrowPitch, narrow_two, s.even_narrow);
+    at_c.template fetch<In::kNarrow>(cc, m, In::kNarrowPitch, narrow_two, s.even_narrow);
+  };
+#pragma unroll
+  for (int k = 0; k < In::kPairs; ++k) u[k] = delta[k] = z[k] = Two<T>{};
+#pragma unroll
+  for (int k = 0; k < In::kNarrow; ++k) bb[k] = cc[k] = Two<T>{};
+  int steps = (int)(p.last - p.first < kTile ? p.last - p.first : kTile);
+  prefetch(steps);
   float a[kStates], start[kStates];
 #pragma unroll
   for (int j = 0; j < kStates; ++j) {
@@ -213,97 +260,88 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
   if (on) joined<kLanes, false>(s, p.b, p.chunk, channel, lane, a, start);
   const f2 a0 = pair(a[0], a[1]), a1 = pair(a[2], a[3]);
   f2 h0 = pair(start[0], start[1]), h1 = pair(start[2], start[3]);
-  T* y = out + p.b * s.length * s.channels;
-
-  Two<T> u[In::kPairs], delta[In::kPairs], z[In::kPairs], bb[In::kNarrow], cc[In::kNarrow];
-  auto prefetch = [&](int64_t t0) {
-#pragma unroll
-    for (int k = 0; k < In::kPairs; ++k) {
-      const int64_t t = t0 + In::step(k);
-      if (In::step(k) < kTile && t < p.last) {
-        u[k] = fetch<T>(s.u, p.b, t, p.c0 + In::channel(k), s.channels, s.even);
-        delta[k] = fetch<T>(s.delta, p.b, t, p.c0 + In::channel(k), s.channels, s.even);
-        if (s.z.p != nullptr) z[k] = fetch<T>(s.z, p.b, t, p.c0 + In::channel(k), s.channels, s.even);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < In::kNarrow; ++k) {
-      const int64_t t = t0 + In::narrow_step(k);
-      if (In::narrow_step(k) < kTile && t < p.last) {
-        bb[k] = fetch<T>(s.B, p.b, t, In::state(k), s.states, s.even_narrow);
-        cc[k] = fetch<T>(s.C, p.b, t, In::state(k), s.states, s.even_narrow);
-      }
-    }
-  };
-  float2 skip[In::kPairs], bias[In::kPairs];
-#pragma unroll
-  for (int k = 0; k < In::kPairs; ++k) {
-    skip[k] = two_of(s.D, p.c0 + In::channel(k), s.channels);
-    bias[k] = two_of(s.bias, p.c0 + In::channel(k), s.channels);
-  }
-  if (p.first < p.last) prefetch(p.first);
+  T* y = out + (p.b * s.length + p.first + in.step) * s.channels + p.c0 + in.channel;
+  const int64_t y_pitch = (int64_t)In::kPitch * s.channels, kept_tile = s.batch * s.channels * kLanes;
+  const bool even_out = s.channels % 2 == 0;
+  float4* kept = keep != nullptr && on
+      ? reinterpret_cast<float4*>(keep) + ((p.first / kKeep * s.batch + p.b) * s.channels + channel) * kLanes + lane : nullptr;
+  const float2 skip = two_of(s.D, p.c0 + in.channel, s.channels), bias = two_of(s.bias, p.c0 + in.channel, s.channels);
+  float4* put_dt = s_dt + in.step * kWide + in.channel;
+  float* put_bc = reinterpret_cast<float*>(s_bc) + in.narrow_step * 2 * kPadded + in.state / kStates * 2 * kStates + in.state % kStates;
+  const float* from_y = s_y + in.step * kLanes * In::kRow + in.channel;
+  const ulonglong2* bc2 = reinterpret_cast<const ulonglong2*>(s_bc) + lane * 2;
+  const ulonglong2* dt2 = reinterpret_cast<const ulonglong2*>(s_dt) + c;
+  float* put_y = s_y + lane * In::kRow + c;
   for (int64_t t0 = p.first; t0 < p.last; t0 += kTile) {
-    const int steps = (int)(p.last - t0 < kTile ? p.last - t0 : kTile);
     float2 du[In::kPairs], gate[In::kPairs];             // D u and silu(z) of the tile, for its end
 #pragma unroll
     for (int k = 0; k < In::kPairs; ++k) {
-      if (In::step(k) >= steps) continue;
+      if (in.step + k * In::kPitch >= steps) continue;
       const float2 uv = u[k].get(), dv = delta[k].get();
-      const float x = dv.x + bias[k].x, w = dv.y + bias[k].y;
+      const float x = dv.x + bias.x, w = dv.y + bias.y;
       const float tx = s.softplus ? softplus(x) : x, tw = s.softplus ? softplus(w) : w;
-      float4* to = s_dt + In::step(k) * kWide + In::channel(k);
-      to[0] = make_float4(tx, tx, tx * uv.x, tx * uv.x);
-      to[1] = make_float4(tw, tw, tw * uv.y, tw * uv.y);
-      du[k] = make_float2(skip[k].x * uv.x, skip[k].y * uv.y);
+      put_dt[k * In::kPitch * kWide] = make_float4(tx, tx, tx * uv.x, tx * uv.x);
+      put_dt[k * In::kPitch * kWide + 1] = make_float4(tw, tw, tw * uv.y, tw * uv.y);
+      du[k] = make_float2(skip.x * uv.x, skip.y * uv.y);
       gate[k] = make_float2(1.0f, 1.0f);
-      if (s.z.p != nullptr) {
+      if (gated) {
         const float2 zv = z[k].get();
         gate[k] = make_float2(activate<kActSilu>(zv.x), activate<kActSilu>(zv.y));
       }
     }
-    float* bc = reinterpret_cast<float*>(s_bc);
 #pragma unroll
     for (int k = 0; k < In::kNarrow; ++k) {
-      if (In::narrow_step(k) >= steps) continue;
-      const int n = In::state(k);
-      float* to = bc + In::narrow_step(k) * 2 * kPadded + n / kStates * 2 * kStates + n % kStates;
-      *reinterpret_cast<float2*>(to) = bb[k].get();
-      *reinterpret_cast<float2*>(to + kStates) = cc[k].get();
+      if (in.narrow_step + k * In::kNarrowPitch >= steps) continue;
+      *reinterpret_cast<float2*>(put_bc + k * In::kNarrowPitch * 2 * kPadded) = bb[k].get();
+      *reinterpret_cast<float2*>(put_bc + k * In::kNarrowPitch * 2 * kPadded + kStates) = cc[k].get();
     }
     __syncthreads();
-    if (t0 + kTile < p.last) prefetch(t0 + kTile);
-    const ulonglong2* bc2 = reinterpret_cast<const ulonglong2*>(s_bc) + lane * 2;
-    const ulonglong2* dt2 = reinterpret_cast<const ulonglong2*>(s_dt) + c;
-#pragma unroll 8
-    for (int t = 0; t < steps; ++t) {
-      if (keep != nullptr && t % kKeep == 0 && on) {
-        const float2 x = halves(h0), w = halves(h1);
-        reinterpret_cast<float4*>(keep)[(((t0 + t) / kKeep * s.batch + p.b) * s.channels + channel) * kLanes + lane] =
-            make_float4(x.x, x.y, w.x, w.y);
-      }
+    const int now = steps;
+    steps = (int)(p.last - t0 - kTile < kTile ? p.last - t0 - kTile : kTile);
+    if (steps > 0) prefetch(steps);
+    auto step = [&](int t) {
       const ulonglong2 dt = dt2[t * kWide], b2 = bc2[t * 2 * kLanes], c2 = bc2[t * 2 * kLanes + 1];
       h0 = fma2(exp2_2(mul2(dt.x, a0)), h0, mul2(dt.y, b2.x));
       h1 = fma2(exp2_2(mul2(dt.x, a1)), h1, mul2(dt.y, b2.y));
-      s_y[(t * kLanes + lane) * In::kRow + c] = sum_of(fma2(c2.y, h1, mul2(c2.x, h0)));
+      put_y[t * kLanes * In::kRow] = sum_of(fma2(c2.y, h1, mul2(c2.x, h0)));
+    };
+    auto save = [&]() {
+      if (kept == nullptr) return;
+      const float2 x = halves(h0), w = halves(h1);
+      *kept = make_float4(x.x, x.y, w.x, w.y);
+      kept += kept_tile;
+    };
+    if (now == kTile) {
+#pragma unroll
+      for (int t = 0; t < kTile; ++t) {
+        if (t % kKeep == 0) save();
+        step(t);
+      }
+    } else {
+      for (int t = 0; t < now; ++t) {
+        if (t % kKeep == 0) save();
+        step(t);
+      }
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < In::kPairs; ++k) {
-      if (In::step(k) >= steps) continue;
-      const float* from = s_y + In::step(k) * kLanes * In::kRow + In::channel(k);
+      if (in.step + k * In::kPitch >= now) continue;
       float v = 0.0f, w = 0.0f;
 #pragma unroll
       for (int l = 0; l < kLanes; ++l) {
-        const float2 part = *reinterpret_cast<const float2*>(from + l * In::kRow);
+        const float2 part = *reinterpret_cast<const float2*>(from_y + (k * In::kPitch * kLanes + l) * In::kRow);
         v += part.x;
         w += part.y;
       }
-      put<T>(y + (t0 + In::step(k)) * s.channels, p.c0 + In::channel(k), s.channels, s.channels % 2 == 0, (v + du[k].x) * gate[k].x,
-             (w + du[k].y) * gate[k].y);
+      put<T>(y + k * y_pitch, 0, two, even_out, (v + du[k].x) * gate[k].x, (w + du[k].y) * gate[k].y);
     }
+    y += (int64_t)kTile * s.channels;
   }
-  for (int64_t t = (p.first > p.len ? p.first : p.len) + threadIdx.x / (kWide / 2); t < p.end; t += kThreads / (kWide / 2))
-    put<T>(y + t * s.channels, p.c0 + threadIdx.x % (kWide / 2) * 2, s.channels, s.channels % 2 == 0, 0.0f, 0.0f);
+  // behind the end: the rows of the chunk that are left
+  T* rest = out + p.b * s.length * s.channels + p.c0 + in.channel;
+  for (int64_t t = (p.first > p.len ? p.first : p.len) + in.step; t < p.end; t += In::kPitch)
+    put<T>(rest + t * s.channels, 0, two, even_out, 0.0f, 0.0f);
   // the chunk that the sequence ends in
   if (state_out != nullptr && on && (p.first < p.len || p.chunk == 0) && p.end >= p.len) {
     const float2 x = halves(h0), w = halves(h1);
@@ -320,13 +358,39 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
 template <class T, int kLanes, bool kReverse>
 __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, const T* __restrict__ dout) {
   pdl_enter();
-  using In = Ahead<T, kLanes>;
+  using In = Lanes<kLanes>;
   constexpr int kWide = In::kWide, kPadded = In::kPadded;
   __shared__ float4 s_bc[kTile * kLanes];                  // B, or C
   __shared__ float4 s_dt[kTile * kWide];                   // dt twice, dt * u (or dy) twice
   const Block<kWide> p(s);
+  const In in;
   const int c = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, channel = p.c0 + c;
-  const bool on = channel < s.channels;
+  const bool on = channel < s.channels, gated = kReverse && s.z.p != nullptr;
+  const int two = left_of(s.channels, p.c0 + in.channel), narrow_two = left_of(s.states, in.state);
+  const int64_t tiles = p.first < p.last ? (p.last - p.first + kTile - 1) / kTile : 0;
+  const int64_t t1 = p.first + (kReverse && tiles > 0 ? tiles - 1 : 0) * kTile;        // the first tile to do
+  constexpr int kStep = kReverse ? -kTile : kTile;
+  Cursor<T> at_x, at_delta, at_z, at_bc;
+  const Seq x_of = kReverse ? Seq{dout, s.length * s.channels, s.channels} : s.u;
+  at_x.set(x_of, p.b, t1 + in.step, p.c0 + in.channel, In::kPitch, kStep);
+  at_delta.set(s.delta, p.b, t1 + in.step, p.c0 + in.channel, In::kPitch, kStep);
+  at_z.set(s.z, p.b, t1 + in.step, p.c0 + in.channel, In::kPitch, kStep);
+  at_bc.set(kReverse ? s.C : s.B, p.b, t1 + in.narrow_step, in.state, In::kNarrowPitch, kStep);
+  Two<T> x[In::kPairs], delta[In::kPairs], z[In::kPairs], bc[In::kNarrow];
+#pragma unroll
+  for (int k = 0; k < In::kPairs; ++k) x[k] = delta[k] = z[k] = Two<T>{};
+#pragma unroll
+  for (int k = 0; k < In::kNarrow; ++k) bc[k] = Two<T>{};
+  const bool even_x = kReverse ? s.channels % 2 == 0 : s.even != 0;
+  auto prefetch = [&](int steps) {
+    const int n = steps - in.step, m = steps - in.narrow_step;
+    at_x.template fetch<In::kPairs>(x, n, In::kPitch, two, even_x);
+    at_delta.template fetch<In::kPairs>(delta, n, In::kPitch, two, s.even);
+    if (gated) at_z.template fetch<In::kPairs>(z, n, In::kPitch, two, s.even);
+    at_bc.template fetch<In::kNarrow>(bc, m, In::kNarrowPitch, narrow_two, s.even_narrow);
+  };
+  int steps = (int)(p.last - t1 < kTile ? p.last - t1 : kTile);
+  if (tiles > 0) prefetch(steps);
   float a[kStates], span = 0.0f;
 #pragma unroll
   for (int j = 0; j < kStates; ++j) {
@@ -335,46 +399,22 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
   }
   const f2 a0 = pair(a[0], a[1]), a1 = pair(a[2], a[3]);
   f2 h0 = 0, h1 = 0;
-  Two<T> x[In::kPairs], delta[In::kPairs], z[In::kPairs], bc[In::kNarrow];
-  auto prefetch = [&](int64_t t0) {
-#pragma unroll
-    for (int k = 0; k < In::kPairs; ++k) {
-      const int64_t t = t0 + In::step(k);
-      const int ch = p.c0 + In::channel(k);
-      if (In::step(k) < kTile && t < p.last) {
-        delta[k] = fetch<T>(s.delta, p.b, t, ch, s.channels, s.even);
-        if constexpr (kReverse) {
-          x[k] = fetch<T>(dout + (p.b * s.length + t) * s.channels, ch, s.channels, s.channels % 2 == 0);
-          if (s.z.p != nullptr) z[k] = fetch<T>(s.z, p.b, t, ch, s.channels, s.even);
-        } else {
-          x[k] = fetch<T>(s.u, p.b, t, ch, s.channels, s.even);
-        }
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < In::kNarrow; ++k) {
-      const int64_t t = t0 + In::narrow_step(k);
-      if (In::narrow_step(k) < kTile && t < p.last) bc[k] = fetch<T>(kReverse ? s.C : s.B, p.b, t, In::state(k), s.states, s.even_narrow);
-    }
-  };
-  float2 bias[In::kPairs];
-#pragma unroll
-  for (int k = 0; k < In::kPairs; ++k) bias[k] = two_of(s.bias, p.c0 + In::channel(k), s.channels);
-  const int64_t tiles = p.first < p.last ? (p.last - p.first + kTile - 1) / kTile : 0;
-  if (tiles > 0) prefetch(p.first + (kReverse ? tiles - 1 : 0) * kTile);
+  const float2 bias = two_of(s.bias, p.c0 + in.channel, s.channels);
+  float4* put_dt = s_dt + in.step * kWide + in.channel;
+  float* put_bc = reinterpret_cast<float*>(s_bc) + in.narrow_step * kPadded + in.state;
+  const ulonglong2* bc2 = reinterpret_cast<const ulonglong2*>(s_bc) + lane;
+  const ulonglong2* dt2 = reinterpret_cast<const ulonglong2*>(s_dt) + c;
   for (int64_t i = 0; i < tiles; ++i) {
-    const int64_t t0 = p.first + (kReverse ? tiles - 1 - i : i) * kTile;
-    const int steps = (int)(p.last - t0 < kTile ? p.last - t0 : kTile);
     if (i > 0) __syncthreads();
 #pragma unroll
     for (int k = 0; k < In::kPairs; ++k) {
-      if (In::step(k) >= steps) continue;
+      if (in.step + k * In::kPitch >= steps) continue;
       float2 v = x[k].get();
       const float2 dv = delta[k].get();
-      const float e = dv.x + bias[k].x, w = dv.y + bias[k].y;
+      const float e = dv.x + bias.x, w = dv.y + bias.y;
       const float te = s.softplus ? softplus(e) : e, tw = s.softplus ? softplus(w) : w;
       if constexpr (kReverse) {
-        if (s.z.p != nullptr) {
+        if (gated) {
           const float2 zv = z[k].get();
           v.x *= activate<kActSilu>(zv.x);
           v.y *= activate<kActSilu>(zv.y);
@@ -383,21 +423,19 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
         v.x *= te;
         v.y *= tw;
       }
-      float4* to = s_dt + In::step(k) * kWide + In::channel(k);
-      to[0] = make_float4(te, te, v.x, v.x);
-      to[1] = make_float4(tw, tw, v.y, v.y);
+      put_dt[k * In::kPitch * kWide] = make_float4(te, te, v.x, v.x);
+      put_dt[k * In::kPitch * kWide + 1] = make_float4(tw, tw, v.y, v.y);
     }
 #pragma unroll
     for (int k = 0; k < In::kNarrow; ++k)
-      if (In::narrow_step(k) < steps)
-        *reinterpret_cast<float2*>(reinterpret_cast<float*>(s_bc) + In::narrow_step(k) * kPadded + In::state(k)) = bc[k].get();
+      if (in.narrow_step + k * In::kNarrowPitch < steps) *reinterpret_cast<float2*>(put_bc + k * In::kNarrowPitch * kPadded) = bc[k].get();
     __syncthreads();
-    if (i + 1 < tiles) prefetch(kReverse ? t0 - kTile : t0 + kTile);
-    const ulonglong2* bc2 = reinterpret_cast<const ulonglong2*>(s_bc) + lane;
-    const ulonglong2* dt2 = reinterpret_cast<const ulonglong2*>(s_dt) + c;
-#pragma unroll 4
-    for (int k = 0; k < steps; ++k) {
-      const int t = kReverse ? steps - 1 - k : k;
+    const int now = steps;
+    const int64_t after = p.first + (kReverse ? tiles - 2 - i : i + 1) * kTile;
+    steps = (int)(p.last - after < kTile ? p.last - after : kTile);
+    if (i + 1 < tiles) prefetch(steps);
+    float sum = 0.0f;
+    auto step = [&](int t) {
       const ulonglong2 dt = dt2[t * kWide], b2 = bc2[t * kLanes];
       const f2 e0 = exp2_2(mul2(dt.x, a0)), e1 = exp2_2(mul2(dt.x, a1));
       if constexpr (kReverse) {
@@ -407,8 +445,15 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
         h0 = fma2(e0, h0, mul2(dt.y, b2.x));
         h1 = fma2(e1, h1, mul2(dt.y, b2.y));
       }
-      span += halves(dt.x).x;
+      sum += halves(dt.x).x;
+    };
+    if (now == kTile) {
+#pragma unroll
+      for (int t = 0; t < kTile; ++t) step(kReverse ? kTile - 1 - t : t);
+    } else {
+      for (int t = 0; t < now; ++t) step(kReverse ? now - 1 - t : t);
     }
+    span += sum;
   }
   if (!on) return;
   const int64_t at = (p.chunk * s.batch + p.b) * s.channels + channel;
@@ -463,6 +508,8 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
   constexpr int kWarps = kThreads / 32, kWide = 8 * kWarps / kBlocks, kPadded = 16 * kBlocks, kSlots = 8 * kBlocks;
   constexpr int kRow = kWide + 4;                            // a warp's eight slots of four channels fall into banks of their own
   constexpr bool kFine = sizeof(T) == 4;
+  using In = Share<kKeep, kWide, kPadded>;
+  static_assert(In::kPairs == 1, "a thread finishes what it has prepared, out of registers");
   __shared__ float4 s_bc[kKeep][kSlots];                     // B of states n and n + 8, C of them
   __shared__ float4 s_dt[kKeep][kWide];                      // dt twice, dt u twice
   __shared__ __align__(16) float2 s_dy[kKeep][kWide];                      // dy twice
@@ -493,75 +540,78 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
     A2[i] = pair(v[0] * kLog2e, v[1] * kLog2e);
     carry[i] = pair(c[0], c[1]);
   }
-  // what a thread prepares and finishes: two channels of a step
-  constexpr int kPairs = kWide / 2;
-  const int pt = threadIdx.x / kPairs, pc = threadIdx.x % kPairs * 2, channel = p.c0 + pc;
-  const bool mine = pt < kKeep;
-  // ... and what it prepares of B (the first half of the threads' turns) and C
-  constexpr int kNarrow = kKeep * kPadded / 2 <= kThreads ? 1 : kKeep * kPadded / 2 / kThreads;
-  const float2 skip = two_of(s.D, channel, s.channels), bias = two_of(s.bias, channel, s.channels);
+  // a thread prepares and finishes two channels of a step, and prepares some of B and C
+  const In in;
+  const int two = left_of(s.channels, p.c0 + in.channel), narrow_two = left_of(s.states, in.state);
+  const bool mine = in.step < kKeep, gated = s.z.p != nullptr, even = s.channels % 2 == 0;
+  const float2 skip = two_of(s.D, p.c0 + in.channel, s.channels), bias = two_of(s.bias, p.c0 + in.channel, s.channels);
   float2 dD = make_float2(0.0f, 0.0f), dbias = dD;
-  const int even = s.channels % 2 == 0;
-  const int64_t base = p.b * s.length;
-  Two<T> u, delta, z, up, bb[kNarrow], cc[kNarrow];
+  const int64_t tiles = p.first < p.last ? (p.last - p.first + kKeep - 1) / kKeep : 0;
+  const int64_t t1 = p.first + (tiles > 0 ? tiles - 1 : 0) * kKeep;
+  Cursor<T> at_u, at_delta, at_z, at_up, at_b, at_c;
+  at_u.set(s.u, p.b, t1 + in.step, p.c0 + in.channel, 0, -kKeep);
+  at_delta.set(s.delta, p.b, t1 + in.step, p.c0 + in.channel, 0, -kKeep);
+  at_z.set(s.z, p.b, t1 + in.step, p.c0 + in.channel, 0, -kKeep);
+  at_up.set({g.dout, s.length * s.channels, s.channels}, p.b, t1 + in.step, p.c0 + in.channel, 0, -kKeep);
+  at_b.set(s.B, p.b, t1 + in.narrow_step, in.state, In::kNarrowPitch, -kKeep);
+  at_c.set(s.C, p.b, t1 + in.narrow_step, in.state, In::kNarrowPitch, -kKeep);
+  const float* at_kept = g.keep + ((t1 / kKeep * s.batch + p.b) * s.channels + ch[0]) * g.kept + n0;
+  const int64_t kept_tile = s.batch * s.channels * g.kept;
+  Two<T> u[1] = {}, delta[1] = {}, z[1] = {}, up[1] = {}, bb[In::kNarrow] = {}, cc[In::kNarrow] = {};
   float kept[2][2];
-  auto prefetch = [&](int64_t t0) {
-    if (mine && t0 + pt < p.last) {
-      u = fetch<T>(s.u, p.b, t0 + pt, channel, s.channels, s.even);
-      delta = fetch<T>(s.delta, p.b, t0 + pt, channel, s.channels, s.even);
-      if (s.z.p != nullptr) z = fetch<T>(s.z, p.b, t0 + pt, channel, s.channels, s.even);
-      up = fetch<T>(reinterpret_cast<const T*>(g.dout) + (base + t0 + pt) * s.channels, channel, s.channels, even);
-    }
-#pragma unroll
-    for (int k = 0; k < kNarrow; ++k) {
-      const int i = threadIdx.x + k * kThreads, t = i / (kPadded / 2), n = i % (kPadded / 2) * 2;
-      if (t < kKeep && t0 + t < p.last) {
-        bb[k] = fetch<T>(s.B, p.b, t0 + t, n, s.states, s.even_narrow);
-        cc[k] = fetch<T>(s.C, p.b, t0 + t, n, s.states, s.even_narrow);
-      }
-    }
+  auto prefetch = [&](int steps) {
+    const int n = mine ? steps - in.step : 0, m = steps - in.narrow_step;
+    at_u.template fetch<1>(u, n, 0, two, s.even);
+    at_delta.template fetch<1>(delta, n, 0, two, s.even);
+    if (gated) at_z.template fetch<1>(z, n, 0, two, s.even);
+    at_up.template fetch<1>(up, n, 0, two, even);
+    at_b.template fetch<In::kNarrow>(bb, m, In::kNarrowPitch, narrow_two, s.even_narrow);
+    at_c.template fetch<In::kNarrow>(cc, m, In::kNarrowPitch, narrow_two, s.even_narrow);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int n = n0 + 8 * j;
-        kept[i][j] = ch[i] < s.channels && n < s.states ? g.keep[((t0 / kKeep * s.batch + p.b) * s.channels + ch[i]) * g.kept + n] : 0.0f;
-      }
+      for (int j = 0; j < 2; ++j)
+        kept[i][j] = ch[i] < s.channels && n0 + 8 * j < s.states ? at_kept[4 * i * g.kept + 8 * j] : 0.0f;
+    at_kept -= kept_tile;
   };
-  const int64_t tiles = p.first < p.last ? (p.last - p.first + kKeep - 1) / kKeep : 0;
-  if (tiles > 0) prefetch(p.first + (tiles - 1) * kKeep);
+  int steps = (int)(p.last - t1 < kKeep ? p.last - t1 : kKeep);
+  if (tiles > 0) prefetch(steps);
+  const int64_t first_row = (p.b * s.length + t1 + in.step) * s.channels + p.c0 + in.channel, rows = (int64_t)kKeep * s.channels;
+  T *to_du = reinterpret_cast<T*>(g.du) + first_row, *to_ddelta = reinterpret_cast<T*>(g.ddelta) + first_row;
+  T* to_dz = g.dz != nullptr ? reinterpret_cast<T*>(g.dz) + first_row : nullptr;
+  float* to_narrow = g.narrow + ((p.block * s.batch + p.b) * s.length + t1) * 2 * kPadded + threadIdx.x;
   for (int64_t tile = tiles - 1; tile >= 0; --tile) {
-    const int64_t t0 = p.first + tile * kKeep;
-    const int steps = (int)(p.last - t0 < kKeep ? p.last - t0 : kKeep);
+    const int now = steps;
+    steps = kKeep;                 // of the tiles ahead of the last one
     // prepare; steps behind the end do nothing: dt = 0 and dy = 0
     float2 uv = make_float2(0.0f, 0.0f), dt = uv, slope_dt = uv, dz = uv, dy = uv;
     if (mine) {
-      if (pt < steps) {
-        const float2 dv = delta.get(), ov = up.get();
-        uv = u.get();
+      if (in.step < now) {
+        const float2 dv = delta[0].get(), ov = up[0].get();
+        uv = u[0].get();
         const float x = dv.x + bias.x, w = dv.y + bias.y;
         dt = make_float2(x, w);
         slope_dt = make_float2(1.0f, 1.0f);
         if (s.softplus) dt = make_float2(softplus(x, &slope_dt.x), softplus(w, &slope_dt.y));
         dy = ov;
-        if (s.z.p != nullptr) {
-          const float2 zv = z.get();
+        if (gated) {
+          const float2 zv = z[0].get();
           const float gx = sigmoid(zv.x), gw = sigmoid(zv.y);
           dy = make_float2(ov.x * zv.x * gx, ov.y * zv.y * gw);
           dz = make_float2(ov.x * gx * (1.0f + zv.x * (1.0f - gx)), ov.y * gw * (1.0f + zv.y * (1.0f - gw)));
         }
       }
-      s_dt[pt][pc] = make_float4(dt.x, dt.x, dt.x * uv.x, dt.x * uv.x);
-      s_dt[pt][pc + 1] = make_float4(dt.y, dt.y, dt.y * uv.y, dt.y * uv.y);
-      *reinterpret_cast<float4*>(&s_dy[pt][pc]) = make_float4(dy.x, dy.x, dy.y, dy.y);
+      s_dt[in.step][in.channel] = make_float4(dt.x, dt.x, dt.x * uv.x, dt.x * uv.x);
+      s_dt[in.step][in.channel + 1] = make_float4(dt.y, dt.y, dt.y * uv.y, dt.y * uv.y);
+      *reinterpret_cast<float4*>(&s_dy[in.step][in.channel]) = make_float4(dy.x, dy.x, dy.y, dy.y);
     }
 #pragma unroll
-    for (int k = 0; k < kNarrow; ++k) {
-      const int i = threadIdx.x + k * kThreads, t = i / (kPadded / 2), n = i % (kPadded / 2) * 2;
+    for (int k = 0; k < In::kNarrow; ++k) {
+      const int t = in.narrow_step + k * In::kNarrowPitch;
       if (t >= kKeep) continue;
-      const float2 zero = make_float2(0.0f, 0.0f), bv = t < steps ? bb[k].get() : zero, cv = t < steps ? cc[k].get() : zero;
+      const float2 zero = make_float2(0.0f, 0.0f), bv = t < now ? bb[k].get() : zero, cv = t < now ? cc[k].get() : zero;
       // states n, n + 1 of sixteen: slots n % 8 and the next, the first or second of each
-      float* to = reinterpret_cast<float*>(&s_bc[t][n / 16 * 8 + n % 8]) + n % 16 / 8;
+      float* to = reinterpret_cast<float*>(&s_bc[t][in.state / 16 * 8 + in.state % 8]) + in.state % 16 / 8;
       to[0] = bv.x;
       to[2] = cv.x;
       to[4] = bv.y;
@@ -571,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
     h[0][0] = pair(kept[0][0], kept[0][1]);
     h[0][1] = pair(kept[1][0], kept[1][1]);
     __syncthreads();
-    if (tile > 0) prefetch(t0 - kKeep);
+    if (tile > 0) prefetch(kKeep);
 #pragma unroll
     for (int t = 0; t < kKeep; ++t) {
       const f2 b = *reinterpret_cast<const f2*>(&s_bc[t][slot]);
@@ -627,43 +677,49 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
       s_narrow[group][1][2 * (lane % 4) + q % 2][n0 + q / 2 * 8] = dC[q];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < steps * 2 * kPadded; i += kThreads) {
-      const int t = i / (2 * kPadded), k = i / kPadded % 2, n = i % kPadded;
+#pragma unroll
+    for (int j = 0; j < kKeep * 2 * kPadded / kThreads; ++j) {
+      const unsigned i = threadIdx.x + j * kThreads, t = i / (2 * kPadded), k = i / kPadded % 2, n = i % kPadded;
+      if ((int)t >= now) break;
       float v = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps / kBlocks; ++w) v += s_narrow[w][k][t][n];
-      g.narrow[((p.block * s.batch + p.b) * s.length + t0) * 2 * kPadded + i] = v;
+      to_narrow[j * kThreads] = v;
     }
-    if (mine && pt < steps) {
+    to_narrow -= kKeep * 2 * kPadded;
+    if (mine && in.step < now) {
       float2 v[3];
 #pragma unroll
       for (int q = 0; q < 3; ++q) {
         float x = 0.0f, w = 0.0f;
 #pragma unroll
         for (int l = 0; l < kSlots; ++l) {
-          const float2 o = *reinterpret_cast<const float2*>(&s_part[q][pt][l][pc]);
+          const float2 o = *reinterpret_cast<const float2*>(&s_part[q][in.step][l][in.channel]);
           x += o.x;
           w += o.y;
         }
         v[q] = make_float2(x, w);
       }
-      const int64_t row = (base + t0 + pt) * s.channels;
-      if (g.dz != nullptr)
-        put<T>(reinterpret_cast<T*>(g.dz) + row, channel, s.channels, even, dz.x * fmaf(skip.x, uv.x, v[0].x), dz.y * fmaf(skip.y, uv.y, v[0].y));
-      put<T>(reinterpret_cast<T*>(g.du) + row, channel, s.channels, even, fmaf(v[1].x, dt.x, skip.x * dy.x), fmaf(v[1].y, dt.y, skip.y * dy.y));
+      if (to_dz != nullptr) put<T>(to_dz, 0, two, even, dz.x * fmaf(skip.x, uv.x, v[0].x), dz.y * fmaf(skip.y, uv.y, v[0].y));
+      put<T>(to_du, 0, two, even, fmaf(v[1].x, dt.x, skip.x * dy.x), fmaf(v[1].y, dt.y, skip.y * dy.y));
       const float ex = fmaf(v[1].x, uv.x, v[2].x) * slope_dt.x, ew = fmaf(v[1].y, uv.y, v[2].y) * slope_dt.y;
-      put<T>(reinterpret_cast<T*>(g.ddelta) + row, channel, s.channels, even, ex, ew);
+      put<T>(to_ddelta, 0, two, even, ex, ew);
       dD.x = fmaf(dy.x, uv.x, dD.x);
       dD.y = fmaf(dy.y, uv.y, dD.y);
       dbias.x += ex;
       dbias.y += ew;
     }
+    to_du -= rows;
+    to_ddelta -= rows;
+    if (to_dz != nullptr) to_dz -= rows;
   }
-  for (int64_t t = (p.first > p.len ? p.first : p.len) + pt; t < p.end; t += kThreads / kPairs) {
-    const int64_t row = (base + t) * s.channels;
-    put<T>(reinterpret_cast<T*>(g.du) + row, channel, s.channels, even, 0.0f, 0.0f);
-    put<T>(reinterpret_cast<T*>(g.ddelta) + row, channel, s.channels, even, 0.0f, 0.0f);
-    if (g.dz != nullptr) put<T>(reinterpret_cast<T*>(g.dz) + row, channel, s.channels, even, 0.0f, 0.0f);
+  // behind the end: the rows of the chunk that are left
+  const int64_t lead = p.b * s.length * s.channels + p.c0 + in.channel;
+  for (int64_t t = (p.first > p.len ? p.first : p.len) + in.step; t < p.end; t += In::kPitch) {
+    const int64_t row = lead + t * s.channels;
+    put<T>(reinterpret_cast<T*>(g.du) + row, 0, two, even, 0.0f, 0.0f);
+    put<T>(reinterpret_cast<T*>(g.ddelta) + row, 0, two, even, 0.0f, 0.0f);
+    if (g.dz != nullptr) put<T>(reinterpret_cast<T*>(g.dz) + row, 0, two, even, 0.0f, 0.0f);
   }
   float* sums = g.sums + (p.b * s.chunks + p.chunk) * (int64_t)s.channels * (s.states + 2);
 #pragma unroll
@@ -675,15 +731,15 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
   float4* stage = reinterpret_cast<float4*>(&s_part[0][0][0][0]);      // room for one of each thread
   stage[threadIdx.x] = make_float4(dD.x, dD.y, dbias.x, dbias.y);
   __syncthreads();
-  if (threadIdx.x < kPairs) {
+  if (threadIdx.x < kWide / 2) {
     float4 v = stage[threadIdx.x];
-    for (int k = threadIdx.x + kPairs; k < kThreads; k += kPairs) {
+    for (int k = threadIdx.x + kWide / 2; k < kThreads; k += kWide / 2) {
       const float4 w = stage[k];
       v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
     }
     float* to = sums + (int64_t)s.channels * s.states;
-    put<float>(to, channel, s.channels, 0, v.x, v.y);
-    put<float>(to + s.channels, channel, s.channels, 0, v.z, v.w);
+    put<float>(to + p.c0 + in.channel, 0, two, false, v.x, v.y);
+    put<float>(to + s.channels + p.c0 + in.channel, 0, two, false, v.z, v.w);
   }
 }
 
@@ -762,7 +818,7 @@ constexpr int64_t kShortest = 128;
 template <class T, int kLanes> int forward(const Scan& s, void* out, float* state_out, float* keep, void* stream) {
   static SmemAllowed allowed{0};
   constexpr int kWide = kThreads / kLanes;
-  constexpr size_t kSmem = kTile * (2 * kLanes * 16 + kWide * 16 + kLanes * Ahead<T, kLanes>::kRow * 4);
+  constexpr size_t kSmem = kTile * (2 * kLanes * 16 + kWide * 16 + kLanes * Lanes<kLanes>::kRow * 4);
   if (kSmem > 48 * 1024) {
     const int rc = allow_smem(selective_scan_fwd_kernel<T, kLanes>, kSmem, allowed);
     if (rc != 0) return rc;
