@@ -10,12 +10,13 @@
 //   ddt = sum_n A a h[t - 1] dh + u sum_n B dh,  du = dt sum_n B dh + D dy
 //
 // One exponential a state and step, against some 8 bytes a channel and step: bound by the special function units and the issue of
-// instructions, not by memory.  States stay in registers over the whole sequence, two to a 64-bit register for the paired fp32
-// instructions.  A tile of steps is prepared elementwise (a thread: two neighbouring channels of a step; their operands are fetched
+// instructions, not by memory.  States stay in registers over the whole sequence, those of two neighbouring channels in a 64-bit
+// register for the paired fp32 instructions.  A tile of steps is prepared elementwise (a thread: two neighbouring channels of a step; their operands are fetched
 // a tile ahead), goes through shared memory to the threads that have the states, and comes back for the sums over the states and
 // the gates.
 //
-// Forward: a channel's states lie in kLanes threads, four in each.  Backward: a warp has eight channels and sixteen states, a
+// Forward: two channels' states lie in kLanes threads, two by four in each: with one channel to a thread the reads of B and C out
+// of shared memory (32 bytes a thread and step) took longer than the exponentials.  Backward: a warp has eight channels and sixteen states, a
 // thread two by two of them as the tensor cores' m16n8k8 fragments want them: the sums over the channels that dB and dC are, eight
 // values a thread and step, are two matrix instructions instead of some forty shuffles and additions.  The states ahead of every
 // eighth step are kept by the forward pass, so that the backward pass needs one exponential a state and step as well.
@@ -31,7 +32,7 @@ namespace {
 using namespace esgd;
 
 constexpr int kThreads = 128;
-constexpr int kStates = 4;           // of a thread
+constexpr int kStates = 4;           // of a thread and channel, forward
 constexpr int kTile = 16;            // steps of a tile, forward
 constexpr int kKeep = 8;             // steps between kept states, and of a tile of the backward pass
 constexpr int kMaxChunks = 64;
@@ -128,9 +129,15 @@ __device__ __forceinline__ f2 exp2_2(f2 x) {
   const float2 v = halves(x);
   return pair(exp2_approx(v.x), exp2_approx(v.y));
 }
-__device__ __forceinline__ float sum_of(f2 v) {
-  const float2 h = halves(v);
-  return h.x + h.y;
+__device__ __forceinline__ f2 pair(float2 v) { return pair(v.x, v.y); }
+// Both halves by one factor.
+__device__ __forceinline__ f2 mul2(f2 a, float b) {
+  const float2 v = halves(a);
+  return pair(v.x * b, v.y * b);
+}
+__device__ __forceinline__ f2 fma2(f2 a, float b, f2 c) {
+  const float2 v = halves(a), w = halves(c);
+  return pair(fmaf(v.x, b, w.x), fmaf(v.y, b, w.y));
 }
 
 // A block: a sequence's channels [c0, c0 + kWide) and steps [first, last) of a chunk, as far as the sequence goes.
@@ -193,21 +200,30 @@ template <class T> struct Cursor {
 __device__ __forceinline__ int left_of(int width, int c) { return width - c < 0 ? 0 : width - c > 2 ? 2 : width - c; }
 
 // Forward passes.  A row of partial sums: a warp's channels of every lane fall into banks of their own.
-template <int kLanes> struct Lanes : Share<kTile, kThreads / kLanes, kLanes * kStates> {
-  static constexpr int kRow = kThreads / kLanes + (32 / kLanes - kThreads / kLanes % 32 + 32) % 32;
+template <int kLanes> struct Lanes : Share<kTile, 2 * kThreads / kLanes, kLanes * kStates> {
+  static constexpr int kRow = 2 * kThreads / kLanes + (32 / kLanes - 2 * kThreads / kLanes % 32 + 32) % 32;
 };
 
-// The states that a block begins with: the given one (forward) or none (backward), and the other chunks' joined to it.
+// The states that a thread begins with: those given, and the other chunks' joined to them; of two channels, four states each.
 template <int kLanes, bool kReverse>
-__device__ __forceinline__ void joined(const Scan& s, int64_t b, int chunk, int channel, int lane, const float (&a)[kStates], float (&h)[kStates]) {
-  if (s.chunks <= 1) return;
+__device__ __forceinline__ void joined(const Scan& s, int64_t b, int chunk, int channel, int two, int lane, const f2 (&a)[kStates], f2 (&h)[kStates]) {
   for (int i = kReverse ? s.chunks - 1 : 0; i != chunk; kReverse ? --i : ++i) {
     const int64_t at = (i * s.batch + b) * s.channels + channel;
-    const float span = s.span[at];
-    const float4 l = reinterpret_cast<const float4*>(s.local)[at * kLanes + lane];
-    const float own[4] = {l.x, l.y, l.z, l.w};
+    const f2 span = pair(s.span[at], two > 1 ? s.span[at + 1] : 0.0f);
+    const float4* local = reinterpret_cast<const float4*>(s.local) + at * kLanes + lane;
+    const float4 l = local[0], r = two > 1 ? local[kLanes] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float own[2][4] = {{l.x, l.y, l.z, l.w}, {r.x, r.y, r.z, r.w}};
 #pragma unroll
-    for (int j = 0; j < kStates; ++j) h[j] = fmaf(exp2_approx(span * a[j]), h[j], own[j]);
+    for (int j = 0; j < kStates; ++j) h[j] = fma2(exp2_2(mul2(span, a[j])), h[j], pair(own[0][j], own[1][j]));
+  }
+}
+// A value of two channels' four states each, zero where there is none.
+template <int kLanes> __device__ __forceinline__ void states_of(const float* p, int64_t row, int states, int two, int lane, float factor, f2 (&to)[kStates]) {
+#pragma unroll
+  for (int j = 0; j < kStates; ++j) {
+    const int n = lane * kStates + j;
+    const bool is = p != nullptr && n < states;
+    to[j] = pair(is && two > 0 ? p[row * states + n] * factor : 0.0f, is && two > 1 ? p[(row + 1) * states + n] * factor : 0.0f);
   }
 }
 
@@ -220,12 +236,11 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
   constexpr int kWide = In::kWide, kPadded = In::kPadded;
   extern __shared__ float4 smem4[];
   float4* s_bc = smem4;                                                   // [kTile][kLanes][2]: four of B, four of C
-  float4* s_dt = s_bc + kTile * 2 * kLanes;                               // [kTile][kWide]: dt twice, dt * u twice
-  float* s_y = reinterpret_cast<float*>(s_dt + kTile * kWide);            // [kTile][kLanes][In::kRow]
+  float4* s_dt = s_bc + kTile * 2 * kLanes;                               // [kTile][kWide / 2]: dt of two channels, dt * u of them
+  float* s_y = reinterpret_cast<float*>(s_dt + kTile * kWide / 2);        // [kTile][kLanes][In::kRow]
   const Block<kWide> p(s);
   const In in;
-  const int c = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, channel = p.c0 + c;
-  const bool on = channel < s.channels;
+  const int c = threadIdx.x / kLanes * 2, lane = threadIdx.x % kLanes, channel = p.c0 + c, on = left_of(s.channels, channel);
   const int two = left_of(s.channels, p.c0 + in.channel), narrow_two = left_of(s.states, in.state);
   Cursor<T> at_u, at_delta, at_z, at_b, at_c;
   Two<T> u[In::kPairs], delta[In::kPairs], z[In::kPairs], bb[In::kNarrow], cc[In::kNarrow];
@@ -249,28 +264,21 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
   for (int k = 0; k < In::kNarrow; ++k) bb[k] = cc[k] = Two<T>{};
   int steps = (int)(p.last - p.first < kTile ? p.last - p.first : kTile);
   prefetch(steps);
-  float a[kStates], start[kStates];
-#pragma unroll
-  for (int j = 0; j < kStates; ++j) {
-    const int n = lane * kStates + j;
-    const bool is = on && n < s.states;
-    a[j] = is ? s.A[(int64_t)channel * s.states + n] * kLog2e : 0.0f;
-    start[j] = is && s.state != nullptr ? s.state[(p.b * s.channels + channel) * s.states + n] : 0.0f;
-  }
-  if (on) joined<kLanes, false>(s, p.b, p.chunk, channel, lane, a, start);
-  const f2 a0 = pair(a[0], a[1]), a1 = pair(a[2], a[3]);
-  f2 h0 = pair(start[0], start[1]), h1 = pair(start[2], start[3]);
+  f2 a[kStates], h[kStates];
+  states_of<kLanes>(s.A, channel, s.states, on, lane, kLog2e, a);
+  states_of<kLanes>(s.state, p.b * s.channels + channel, s.states, on, lane, 1.0f, h);
+  if (s.chunks > 1 && on) joined<kLanes, false>(s, p.b, p.chunk, channel, on, lane, a, h);
   T* y = out + (p.b * s.length + p.first + in.step) * s.channels + p.c0 + in.channel;
   const int64_t y_pitch = (int64_t)In::kPitch * s.channels, kept_tile = s.batch * s.channels * kLanes;
   const bool even_out = s.channels % 2 == 0;
-  float4* kept = keep != nullptr && on
+  float4* kept = keep != nullptr && on > 0
       ? reinterpret_cast<float4*>(keep) + ((p.first / kKeep * s.batch + p.b) * s.channels + channel) * kLanes + lane : nullptr;
   const float2 skip = two_of(s.D, p.c0 + in.channel, s.channels), bias = two_of(s.bias, p.c0 + in.channel, s.channels);
-  float4* put_dt = s_dt + in.step * kWide + in.channel;
+  float4* put_dt = s_dt + (in.step * kWide + in.channel) / 2;
   float* put_bc = reinterpret_cast<float*>(s_bc) + in.narrow_step * 2 * kPadded + in.state / kStates * 2 * kStates + in.state % kStates;
   const float* from_y = s_y + in.step * kLanes * In::kRow + in.channel;
-  const ulonglong2* bc2 = reinterpret_cast<const ulonglong2*>(s_bc) + lane * 2;
-  const ulonglong2* dt2 = reinterpret_cast<const ulonglong2*>(s_dt) + c;
+  const float4* bc = s_bc + lane * 2;
+  const ulonglong2* dt2 = reinterpret_cast<const ulonglong2*>(s_dt) + c / 2;
   float* put_y = s_y + lane * In::kRow + c;
   for (int64_t t0 = p.first; t0 < p.last; t0 += kTile) {
     float2 du[In::kPairs], gate[In::kPairs];             // D u and silu(z) of the tile, for its end
@@ -280,8 +288,7 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
       const float2 uv = u[k].get(), dv = delta[k].get();
       const float x = dv.x + bias.x, w = dv.y + bias.y;
       const float tx = s.softplus ? softplus(x) : x, tw = s.softplus ? softplus(w) : w;
-      put_dt[k * In::kPitch * kWide] = make_float4(tx, tx, tx * uv.x, tx * uv.x);
-      put_dt[k * In::kPitch * kWide + 1] = make_float4(tw, tw, tw * uv.y, tw * uv.y);
+      put_dt[k * In::kPitch * kWide / 2] = make_float4(tx, tw, tx * uv.x, tw * uv.y);
       du[k] = make_float2(skip.x * uv.x, skip.y * uv.y);
       gate[k] = make_float2(1.0f, 1.0f);
       if (gated) {
@@ -300,28 +307,30 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
     steps = (int)(p.last - t0 - kTile < kTile ? p.last - t0 - kTile : kTile);
     if (steps > 0) prefetch(steps);
     auto step = [&](int t) {
-      const ulonglong2 dt = dt2[t * kWide], b2 = bc2[t * 2 * kLanes], c2 = bc2[t * 2 * kLanes + 1];
-      h0 = fma2(exp2_2(mul2(dt.x, a0)), h0, mul2(dt.y, b2.x));
-      h1 = fma2(exp2_2(mul2(dt.x, a1)), h1, mul2(dt.y, b2.y));
-      put_y[t * kLanes * In::kRow] = sum_of(fma2(c2.y, h1, mul2(c2.x, h0)));
-    };
-    auto save = [&]() {
-      if (kept == nullptr) return;
-      const float2 x = halves(h0), w = halves(h1);
-      *kept = make_float4(x.x, x.y, w.x, w.y);
-      kept += kept_tile;
+      if (t % kKeep == 0 && kept != nullptr) {
+        float2 v[kStates];
+#pragma unroll
+        for (int j = 0; j < kStates; ++j) v[j] = halves(h[j]);
+        kept[0] = make_float4(v[0].x, v[1].x, v[2].x, v[3].x);
+        if (on > 1) kept[kLanes] = make_float4(v[0].y, v[1].y, v[2].y, v[3].y);
+        kept += kept_tile;
+      }
+      const ulonglong2 dt = dt2[t * kWide / 2];
+      const float4 b4 = bc[t * 2 * kLanes], c4 = bc[t * 2 * kLanes + 1];
+      const float b[kStates] = {b4.x, b4.y, b4.z, b4.w}, c[kStates] = {c4.x, c4.y, c4.z, c4.w};
+      f2 sum = 0;
+#pragma unroll
+      for (int j = 0; j < kStates; ++j) {
+        h[j] = fma2(exp2_2(mul2(dt.x, a[j])), h[j], mul2(dt.y, b[j]));
+        sum = j == 0 ? mul2(h[j], c[j]) : fma2(h[j], c[j], sum);
+      }
+      *reinterpret_cast<f2*>(put_y + t * kLanes * In::kRow) = sum;
     };
     if (now == kTile) {
 #pragma unroll
-      for (int t = 0; t < kTile; ++t) {
-        if (t % kKeep == 0) save();
-        step(t);
-      }
+      for (int t = 0; t < kTile; ++t) step(t);
     } else {
-      for (int t = 0; t < now; ++t) {
-        if (t % kKeep == 0) save();
-        step(t);
-      }
+      for (int t = 0; t < now; ++t) step(t);
     }
     __syncthreads();
 #pragma unroll
@@ -343,15 +352,14 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
   for (int64_t t = (p.first > p.len ? p.first : p.len) + in.step; t < p.end; t += In::kPitch)
     put<T>(rest + t * s.channels, 0, two, even_out, 0.0f, 0.0f);
   // the chunk that the sequence ends in
-  if (state_out != nullptr && on && (p.first < p.len || p.chunk == 0) && p.end >= p.len) {
-    const float2 x = halves(h0), w = halves(h1);
-    const float h[kStates] = {x.x, x.y, w.x, w.y};
+  if (state_out != nullptr && (p.first < p.len || p.chunk == 0) && p.end >= p.len)
 #pragma unroll
     for (int j = 0; j < kStates; ++j) {
       const int n = lane * kStates + j;
-      if (n < s.states) state_out[(p.b * s.channels + channel) * s.states + n] = h[j];
+      float* to = state_out + (p.b * s.channels + channel) * s.states + n;
+      if (n < s.states && on > 0) to[0] = halves(h[j]).x;
+      if (n < s.states && on > 1) to[s.states] = halves(h[j]).y;
     }
-  }
 }
 
 // A chunk by itself, from a state of zero: forward h, or backward the carry a dh that leaves its first step; and the sum of its dt.
@@ -361,11 +369,11 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
   using In = Lanes<kLanes>;
   constexpr int kWide = In::kWide, kPadded = In::kPadded;
   __shared__ float4 s_bc[kTile * kLanes];                  // B, or C
-  __shared__ float4 s_dt[kTile * kWide];                   // dt twice, dt * u (or dy) twice
+  __shared__ float4 s_dt[kTile * kWide / 2];               // of two channels: dt, and dt * u (or dy)
   const Block<kWide> p(s);
   const In in;
-  const int c = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, channel = p.c0 + c;
-  const bool on = channel < s.channels, gated = kReverse && s.z.p != nullptr;
+  const int c = threadIdx.x / kLanes * 2, lane = threadIdx.x % kLanes, channel = p.c0 + c, on = left_of(s.channels, channel);
+  const bool gated = kReverse && s.z.p != nullptr;
   const int two = left_of(s.channels, p.c0 + in.channel), narrow_two = left_of(s.states, in.state);
   const int64_t tiles = p.first < p.last ? (p.last - p.first + kTile - 1) / kTile : 0;
   const int64_t t1 = p.first + (kReverse && tiles > 0 ? tiles - 1 : 0) * kTile;        // the first tile to do
@@ -391,19 +399,14 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
   };
   int steps = (int)(p.last - t1 < kTile ? p.last - t1 : kTile);
   if (tiles > 0) prefetch(steps);
-  float a[kStates], span = 0.0f;
-#pragma unroll
-  for (int j = 0; j < kStates; ++j) {
-    const int n = lane * kStates + j;
-    a[j] = on && n < s.states ? s.A[(int64_t)channel * s.states + n] * kLog2e : 0.0f;
-  }
-  const f2 a0 = pair(a[0], a[1]), a1 = pair(a[2], a[3]);
-  f2 h0 = 0, h1 = 0;
+  f2 a[kStates], h[kStates] = {0, 0, 0, 0};
+  float2 span = make_float2(0.0f, 0.0f);
+  states_of<kLanes>(s.A, channel, s.states, on, lane, kLog2e, a);
   const float2 bias = two_of(s.bias, p.c0 + in.channel, s.channels);
-  float4* put_dt = s_dt + in.step * kWide + in.channel;
+  float4* put_dt = s_dt + (in.step * kWide + in.channel) / 2;
   float* put_bc = reinterpret_cast<float*>(s_bc) + in.narrow_step * kPadded + in.state;
-  const ulonglong2* bc2 = reinterpret_cast<const ulonglong2*>(s_bc) + lane;
-  const ulonglong2* dt2 = reinterpret_cast<const ulonglong2*>(s_dt) + c;
+  const float4* in_bc = s_bc + lane;
+  const ulonglong2* dt2 = reinterpret_cast<const ulonglong2*>(s_dt) + c / 2;
   for (int64_t i = 0; i < tiles; ++i) {
     if (i > 0) __syncthreads();
 #pragma unroll
@@ -423,8 +426,7 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
         v.x *= te;
         v.y *= tw;
       }
-      put_dt[k * In::kPitch * kWide] = make_float4(te, te, v.x, v.x);
-      put_dt[k * In::kPitch * kWide + 1] = make_float4(tw, tw, v.y, v.y);
+      put_dt[k * In::kPitch * kWide / 2] = make_float4(te, tw, v.x, v.y);
     }
 #pragma unroll
     for (int k = 0; k < In::kNarrow; ++k)
@@ -434,18 +436,19 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
     const int64_t after = p.first + (kReverse ? tiles - 2 - i : i + 1) * kTile;
     steps = (int)(p.last - after < kTile ? p.last - after : kTile);
     if (i + 1 < tiles) prefetch(steps);
-    float sum = 0.0f;
+    float2 sum = make_float2(0.0f, 0.0f);
     auto step = [&](int t) {
-      const ulonglong2 dt = dt2[t * kWide], b2 = bc2[t * kLanes];
-      const f2 e0 = exp2_2(mul2(dt.x, a0)), e1 = exp2_2(mul2(dt.x, a1));
-      if constexpr (kReverse) {
-        h0 = mul2(e0, fma2(dt.y, b2.x, h0));
-        h1 = mul2(e1, fma2(dt.y, b2.y, h1));
-      } else {
-        h0 = fma2(e0, h0, mul2(dt.y, b2.x));
-        h1 = fma2(e1, h1, mul2(dt.y, b2.y));
+      const ulonglong2 dt = dt2[t * kWide / 2];
+      const float4 b4 = in_bc[t * kLanes];
+      const float b[kStates] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+      for (int j = 0; j < kStates; ++j) {
+        const f2 e = exp2_2(mul2(dt.x, a[j]));
+        if constexpr (kReverse) h[j] = mul2(e, fma2(dt.y, b[j], h[j]));
+        else h[j] = fma2(e, h[j], mul2(dt.y, b[j]));
       }
-      sum += halves(dt.x).x;
+      sum.x += halves(dt.x).x;
+      sum.y += halves(dt.x).y;
     };
     if (now == kTile) {
 #pragma unroll
@@ -453,13 +456,18 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
     } else {
       for (int t = 0; t < now; ++t) step(kReverse ? now - 1 - t : t);
     }
-    span += sum;
+    span.x += sum.x;
+    span.y += sum.y;
   }
-  if (!on) return;
   const int64_t at = (p.chunk * s.batch + p.b) * s.channels + channel;
-  const float2 v = halves(h0), w = halves(h1);
-  reinterpret_cast<float4*>(s.local)[at * kLanes + lane] = make_float4(v.x, v.y, w.x, w.y);
-  if (lane == 0) s.span[at] = span;
+  float2 v[kStates];
+#pragma unroll
+  for (int j = 0; j < kStates; ++j) v[j] = halves(h[j]);
+  float4* local = reinterpret_cast<float4*>(s.local) + at * kLanes + lane;
+  if (on > 0) local[0] = make_float4(v[0].x, v[1].x, v[2].x, v[3].x);
+  if (on > 1) local[kLanes] = make_float4(v[0].y, v[1].y, v[2].y, v[3].y);
+  if (on > 0 && lane == 0) s.span[at] = span.x;
+  if (on > 1 && lane == 0) s.span[at + 1] = span.y;
 }
 
 struct Grads {
@@ -471,11 +479,8 @@ struct Grads {
   float* sums;                 // [batch][chunks][channels * states + channels + channels]: dA, dD, ddelta_bias
 };
 
-__device__ __forceinline__ uint32_t tf32(float x) {
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return r;
-}
+// The matrix instruction reads eleven bits of a factor: half a step of these more, and leaving the others out rounds to the nearest.
+__device__ __forceinline__ uint32_t tf32(float x) { return __float_as_uint(x) + 0x1000u; }
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -492,54 +497,55 @@ template <bool kFine> __device__ __forceinline__ void product(float (&d)[4], con
   if constexpr (kFine) {
     uint32_t al[4], bl[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) al[i] = tf32(a[i] - __uint_as_float(ah[i]));
+    for (int i = 0; i < 4; ++i) al[i] = tf32(a[i] - __uint_as_float(ah[i] & ~0x1fffu));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) bl[i] = tf32(b[i] - __uint_as_float(bh[i]));
+    for (int i = 0; i < 2; ++i) bl[i] = tf32(b[i] - __uint_as_float(bh[i] & ~0x1fffu));
     mma(d, ah, bl);
     mma(d, al, bh);
   }
 }
 
-// A warp: eight channels and sixteen states.  Thread: channels c and c + 4 (c = lane % 4), states n and n + 8 (n = lane / 4).
+// A warp: eight channels and sixteen states.  Thread: channels 2 c and 2 c + 1 (c = lane % 4, the fragments' columns c and c + 4),
+// states n and n + 8 (n = lane / 4, their rows).
 // kBlocks warps side by side have the states of wider layers.
 template <class T, int kBlocks>
 __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s, Grads g) {
   pdl_enter();
   constexpr int kWarps = kThreads / 32, kWide = 8 * kWarps / kBlocks, kPadded = 16 * kBlocks, kSlots = 8 * kBlocks;
-  constexpr int kRow = kWide + 4;                            // a warp's eight slots of four channels fall into banks of their own
+  constexpr int kRow = kWide == 8 ? 8 : kWide + 8;           // four slots of eight channels fall into banks of their own
   constexpr bool kFine = sizeof(T) == 4;
   using In = Share<kKeep, kWide, kPadded>;
   static_assert(In::kPairs == 1, "a thread finishes what it has prepared, out of registers");
   __shared__ float4 s_bc[kKeep][kSlots];                     // B of states n and n + 8, C of them
-  __shared__ float4 s_dt[kKeep][kWide];                      // dt twice, dt u twice
-  __shared__ __align__(16) float2 s_dy[kKeep][kWide];                      // dy twice
+  __shared__ float4 s_dt[kKeep][kWide / 2];                  // of two channels: dt, and dt u
+  __shared__ f2 s_dy[kKeep][kWide / 2];                      // dy of them
   __shared__ __align__(16) float s_part[3][kKeep][kSlots][kRow];           // C h, B dh, A a h[t - 1] dh of a thread's two states
   __shared__ float s_narrow[kWarps / kBlocks][2][kKeep][kPadded + 4];   // dB, dC over a warp's channels
   const Block<kWide> p(s);
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, part = warp % kBlocks, group = warp / kBlocks;
-  const int slot = part * 8 + lane / 4, n0 = part * 16 + lane / 4, w0 = group * 8 + lane % 4;     // state, channel in the block
-  const int ch[2] = {p.c0 + w0, p.c0 + w0 + 4};
-  f2 A[2], A2[2], carry[2], dA[2];                           // of a channel: its two states
+  const int slot = part * 8 + lane / 4, n0 = part * 16 + lane / 4, w0 = group * 8 + lane % 4 * 2;     // state, channel in the block
+  const int channel = p.c0 + w0, on = left_of(s.channels, channel);
+  f2 A[2], carry[2], dA[2];                                  // of a state: its two channels
   float dA_sum[2][2], dA_low[2][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int j = 0; j < 2; ++j) {
+    const int n = n0 + 8 * j;
     float v[2], c[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int n = n0 + 8 * j;
-      const bool is = ch[i] < s.channels && n < s.states;
-      v[j] = is ? s.A[(int64_t)ch[i] * s.states + n] : 0.0f;
-      dA_sum[i][j] = dA_low[i][j] = 0.0f;
+    for (int i = 0; i < 2; ++i) {
+      const bool is = i < on && n < s.states;
+      v[i] = is ? s.A[(int64_t)(channel + i) * s.states + n] : 0.0f;
+      dA_sum[j][i] = dA_low[j][i] = 0.0f;
       if (is && s.chunks > 1)
         for (int q = s.chunks - 1; q > p.chunk; --q) {
-          const int64_t at = (q * s.batch + p.b) * s.channels + ch[i];
-          c[j] = fmaf(exp2_approx(s.span[at] * (v[j] * kLog2e)), c[j], s.local[at * g.kept + n]);
+          const int64_t at = (q * s.batch + p.b) * s.channels + channel + i;
+          c[i] = fmaf(exp2_approx(s.span[at] * (v[i] * kLog2e)), c[i], s.local[at * g.kept + n]);
         }
     }
-    A[i] = pair(v[0], v[1]);
-    A2[i] = pair(v[0] * kLog2e, v[1] * kLog2e);
-    carry[i] = pair(c[0], c[1]);
+    A[j] = pair(v[0], v[1]);
+    carry[j] = pair(c[0], c[1]);
   }
+  const f2 A2[2] = {mul2(A[0], kLog2e), mul2(A[1], kLog2e)};
   // a thread prepares and finishes two channels of a step, and prepares some of B and C
   const In in;
   const int two = left_of(s.channels, p.c0 + in.channel), narrow_two = left_of(s.states, in.state);
@@ -555,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
   at_up.set({g.dout, s.length * s.channels, s.channels}, p.b, t1 + in.step, p.c0 + in.channel, 0, -kKeep);
   at_b.set(s.B, p.b, t1 + in.narrow_step, in.state, In::kNarrowPitch, -kKeep);
   at_c.set(s.C, p.b, t1 + in.narrow_step, in.state, In::kNarrowPitch, -kKeep);
-  const float* at_kept = g.keep + ((t1 / kKeep * s.batch + p.b) * s.channels + ch[0]) * g.kept + n0;
+  const float* at_kept = g.keep + ((t1 / kKeep * s.batch + p.b) * s.channels + channel) * g.kept + n0;
   const int64_t kept_tile = s.batch * s.channels * g.kept;
   Two<T> u[1] = {}, delta[1] = {}, z[1] = {}, up[1] = {}, bb[In::kNarrow] = {}, cc[In::kNarrow] = {};
   float kept[2][2];
@@ -568,10 +574,9 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
     at_b.template fetch<In::kNarrow>(bb, m, In::kNarrowPitch, narrow_two, s.even_narrow);
     at_c.template fetch<In::kNarrow>(cc, m, In::kNarrowPitch, narrow_two, s.even_narrow);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        kept[i][j] = ch[i] < s.channels && n0 + 8 * j < s.states ? at_kept[4 * i * g.kept + 8 * j] : 0.0f;
+      for (int i = 0; i < 2; ++i) kept[j][i] = i < on && n0 + 8 * j < s.states ? at_kept[i * g.kept + 8 * j] : 0.0f;
     at_kept -= kept_tile;
   };
   int steps = (int)(p.last - t1 < kKeep ? p.last - t1 : kKeep);
@@ -601,9 +606,8 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
           dz = make_float2(ov.x * gx * (1.0f + zv.x * (1.0f - gx)), ov.y * gw * (1.0f + zv.y * (1.0f - gw)));
         }
       }
-      s_dt[in.step][in.channel] = make_float4(dt.x, dt.x, dt.x * uv.x, dt.x * uv.x);
-      s_dt[in.step][in.channel + 1] = make_float4(dt.y, dt.y, dt.y * uv.y, dt.y * uv.y);
-      *reinterpret_cast<float4*>(&s_dy[in.step][in.channel]) = make_float4(dy.x, dy.x, dy.y, dy.y);
+      s_dt[in.step][in.channel / 2] = make_float4(dt.x, dt.y, dt.x * uv.x, dt.y * uv.y);
+      s_dy[in.step][in.channel / 2] = pair(dy);
     }
 #pragma unroll
     for (int k = 0; k < In::kNarrow; ++k) {
@@ -624,51 +628,51 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
     if (tile > 0) prefetch(kKeep);
 #pragma unroll
     for (int t = 0; t < kKeep; ++t) {
-      const f2 b = *reinterpret_cast<const f2*>(&s_bc[t][slot]);
+      const float2 b = *reinterpret_cast<const float2*>(&s_bc[t][slot]);
+      const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(&s_dt[t][w0 / 2]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(&s_dt[t][w0 + 4 * i]);
-        a[t][i] = exp2_2(mul2(d.x, A2[i]));
-        h[t + 1][i] = fma2(a[t][i], h[t][i], mul2(d.y, b));
+      for (int j = 0; j < 2; ++j) {
+        a[t][j] = exp2_2(mul2(d.x, A2[j]));
+        h[t + 1][j] = fma2(a[t][j], h[t][j], mul2(d.y, j == 0 ? b.x : b.y));
       }
     }
+    // step lane / 4 is the column of the fragments that this lane has
+    const float2 own_dy = halves(s_dy[lane / 4][w0 / 2]);
+    const float2 own_du = halves(reinterpret_cast<const ulonglong2*>(&s_dt[lane / 4][w0 / 2])->y);
     float dB[4] = {0, 0, 0, 0}, dC[4] = {0, 0, 0, 0};        // state n (n + 8), steps 2 (lane % 4) and the next
     dA[0] = dA[1] = 0;
 #pragma unroll
     for (int t = kKeep - 1; t >= 0; --t) {
-      const ulonglong2 bc = *reinterpret_cast<const ulonglong2*>(&s_bc[t][slot]);
-      f2 dh[2];
-      float by[2], bu[2];
+      const float4 bc = s_bc[t][slot];
+      const f2 d = *reinterpret_cast<const f2*>(&s_dt[t][w0 / 2]), y2 = s_dy[t][w0 / 2];
+      f2 dh[2], da[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(&s_dt[t][w0 + 4 * i]);
-        const f2 y2 = *reinterpret_cast<const f2*>(&s_dy[t][w0 + 4 * i]);
-        dh[i] = fma2(bc.y, y2, carry[i]);
-        carry[i] = mul2(a[t][i], dh[i]);
-        const f2 da = mul2(carry[i], h[t][i]);
-        dA[i] = fma2(da, d.x, dA[i]);
-        s_part[0][t][slot][w0 + 4 * i] = sum_of(mul2(bc.y, h[t + 1][i]));
-        s_part[1][t][slot][w0 + 4 * i] = sum_of(mul2(bc.x, dh[i]));
-        s_part[2][t][slot][w0 + 4 * i] = sum_of(mul2(da, A[i]));
-        const bool column = lane / 4 == t;
-        by[i] = column ? halves(y2).x : 0.0f;
-        bu[i] = column ? halves(d.y).x : 0.0f;
+      for (int j = 0; j < 2; ++j) {
+        dh[j] = fma2(y2, j == 0 ? bc.z : bc.w, carry[j]);
+        carry[j] = mul2(a[t][j], dh[j]);
+        da[j] = mul2(carry[j], h[t][j]);
+        dA[j] = fma2(da[j], d, dA[j]);
       }
+      *reinterpret_cast<f2*>(&s_part[0][t][slot][w0]) = fma2(h[t + 1][1], bc.w, mul2(h[t + 1][0], bc.z));
+      *reinterpret_cast<f2*>(&s_part[1][t][slot][w0]) = fma2(dh[1], bc.y, mul2(dh[0], bc.x));
+      *reinterpret_cast<f2*>(&s_part[2][t][slot][w0]) = fma2(da[1], A[1], mul2(da[0], A[0]));
+      const bool column = lane / 4 == t;
+      const float by[2] = {column ? own_dy.x : 0.0f, column ? own_dy.y : 0.0f}, bu[2] = {column ? own_du.x : 0.0f, column ? own_du.y : 0.0f};
       const float2 h0 = halves(h[t + 1][0]), h1 = halves(h[t + 1][1]), d0 = halves(dh[0]), d1 = halves(dh[1]);
-      const float ha[4] = {h0.x, h0.y, h1.x, h1.y}, da4[4] = {d0.x, d0.y, d1.x, d1.y};
+      const float ha[4] = {h0.x, h1.x, h0.y, h1.y}, da4[4] = {d0.x, d1.x, d0.y, d1.y};
       product<kFine>(dC, ha, by);
       product<kFine>(dB, da4, bu);
     }
     // into the running sum with its rounding errors beside it: a sequence has thousands of terms
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float2 v = halves(dA[i]);
+    for (int j = 0; j < 2; ++j) {
+      const float2 v = halves(dA[j]);
       const float add[2] = {v.x, v.y};
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float y = add[j] - dA_low[i][j], t = dA_sum[i][j] + y;
-        dA_low[i][j] = (t - dA_sum[i][j]) - y;
-        dA_sum[i][j] = t;
+      for (int i = 0; i < 2; ++i) {
+        const float y = add[i] - dA_low[j][i], t = dA_sum[j][i] + y;
+        dA_low[j][i] = (t - dA_sum[j][i]) - y;
+        dA_sum[j][i] = t;
       }
     }
 #pragma unroll
@@ -723,10 +727,10 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
   }
   float* sums = g.sums + (p.b * s.chunks + p.chunk) * (int64_t)s.channels * (s.states + 2);
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      if (ch[i] < s.channels && n0 + 8 * j < s.states) sums[(int64_t)ch[i] * s.states + n0 + 8 * j] = dA_sum[i][j];
+    for (int i = 0; i < 2; ++i)
+      if (i < on && n0 + 8 * j < s.states) sums[(int64_t)(channel + i) * s.states + n0 + 8 * j] = dA_sum[j][i];
   __syncthreads();
   float4* stage = reinterpret_cast<float4*>(&s_part[0][0][0][0]);      // room for one of each thread
   stage[threadIdx.x] = make_float4(dD.x, dD.y, dbias.x, dbias.y);
@@ -806,19 +810,35 @@ int lanes_of(int states) {
 int state_blocks(int states) { return states <= 16 ? 1 : states <= 32 ? 2 : 4; }
 int blocks_of(int channels, int wide) { return (channels + wide - 1) / wide; }
 
-// Chunks of a pass over `blocks` blocks.  CHUNK_RULE
-void split(Scan* s, int64_t blocks, int64_t shortest) {
-  int64_t n = 1;
-  while (n < kMaxChunks && blocks * n < 2 * sm_count() && s->length / (2 * n) >= shortest) n *= 2;
-  s->chunk = ((s->length + n - 1) / n + kTile - 1) / kTile * kTile;
-  s->chunks = s->chunk > 0 ? (int)((s->length + s->chunk - 1) / s->chunk) : 1;
+// Chunks of a pass over `blocks` blocks, the number that is estimated to take least.  A block takes as long as its steps, a start of
+// some 24 steps, and the chunks ahead of it to join; an SM has `full` blocks at the pace of one, and takes longer with more, up to
+// `most` at a time; with chunks there is a pass more, and all that is done `again` times.  Forward, us without and with them:
+// 1 x 4099 steps of 2048 channels 930 / 129 (29 chunks), 2 x 500 of 4096 146 / 62, 8 x 120 of 2048 26 / 35.
+struct Pace {
+  double full, again;
+  int64_t most;
+};
+constexpr Pace kForward = {4.2, 1.9, 8}, kBackward = {3.0, 1.35, 3};
+void split(Scan* s, int64_t blocks, const Pace& p) {
+  double best = 0.0;
+  for (int64_t n = 1; n <= kMaxChunks; n *= 2) {
+    const int64_t chunk = ((s->length + n - 1) / n + kTile - 1) / kTile * kTile;
+    if (n > 1 && chunk >= s->length) break;
+    const int64_t chunks = chunk > 0 ? (s->length + chunk - 1) / chunk : 1;
+    const int64_t here = (blocks * chunks + sm_count() - 1) / sm_count(), rest = here % p.most;
+    const double pace = (double)(here / p.most) * (double)p.most / p.full + (rest == 0 ? 0.0 : rest < p.full ? 1.0 : (double)rest / p.full);
+    const double cost = (chunks > 1 ? p.again : 1.0) * ((double)chunk + 24.0 + 0.25 * (double)chunks) * pace;
+    if (n > 1 && cost >= best) continue;
+    best = cost;
+    s->chunk = chunk;
+    s->chunks = (int)chunks;
+  }
 }
-constexpr int64_t kShortest = 128;
 
 template <class T, int kLanes> int forward(const Scan& s, void* out, float* state_out, float* keep, void* stream) {
   static SmemAllowed allowed{0};
-  constexpr int kWide = kThreads / kLanes;
-  constexpr size_t kSmem = kTile * (2 * kLanes * 16 + kWide * 16 + kLanes * Lanes<kLanes>::kRow * 4);
+  constexpr int kWide = Lanes<kLanes>::kWide;
+  constexpr size_t kSmem = kTile * (2 * kLanes * 16 + kWide * 8 + kLanes * Lanes<kLanes>::kRow * 4);
   if (kSmem > 48 * 1024) {
     const int rc = allow_smem(selective_scan_fwd_kernel<T, kLanes>, kSmem, allowed);
     if (rc != 0) return rc;
@@ -831,7 +851,7 @@ template <class T, int kLanes> int forward(const Scan& s, void* out, float* stat
   return launch(selective_scan_fwd_kernel<T, kLanes>, grid, kThreads, kSmem, stream, s, (T*)out, state_out, keep);
 }
 template <class T, int kLanes> int carries(const Scan& s, const void* dout, void* stream) {
-  const dim3 grid((unsigned)(s.batch * s.chunks * blocks_of(s.channels, kThreads / kLanes)));
+  const dim3 grid((unsigned)(s.batch * s.chunks * blocks_of(s.channels, Lanes<kLanes>::kWide)));
   return launch(selective_scan_chunk_kernel<T, kLanes, true>, grid, kThreads, 0, stream, s, (const T*)dout);
 }
 template <class T, int kBlocks> int backward_blocks(const Scan& s, const Grads& g, void* dB, void* dC, void* stream) {
@@ -861,7 +881,7 @@ template <class T, int kLanes> int step(const Scan& s, float* state_out, void* o
 
 bool taken(const Scan& s) { return s.states >= 1 && s.states <= 64 && s.channels >= 1 && s.batch >= 0 && s.length >= 0; }
 
-Scan scan_of(const esgd_scan* e) {
+Scan scan_of(const esgd_scan* e, bool backward) {
   Scan s = {};
   Seq* q[5] = {&s.u, &s.delta, &s.z, &s.B, &s.C};
   const uintptr_t size = e->is_bf16 ? 2 : 4;
@@ -876,7 +896,8 @@ Scan scan_of(const esgd_scan* e) {
   s.state = e->state;
   s.batch = e->batch; s.length = e->length;
   s.channels = e->channels; s.states = e->states; s.softplus = e->softplus;
-  split(&s, s.batch * blocks_of(s.channels, kThreads / lanes_of(s.states)), kShortest);
+  if (backward) split(&s, s.batch * blocks_of(s.channels, 32 / state_blocks(s.states)), kBackward);
+  else split(&s, s.batch * blocks_of(s.channels, 2 * kThreads / lanes_of(s.states)), kForward);
   return s;
 }
 int64_t local_floats(const Scan& s) { return s.chunks <= 1 ? 0 : s.chunks * s.batch * s.channels * (lanes_of(s.states) * kStates + 1); }
@@ -890,9 +911,9 @@ void place(Scan* s, float* local) {
 
 extern "C" {
 
-// Floats of room for a pass in either direction (the chunks'; none for many sequences or short ones), for what the forward pass
+// Floats of room for a pass in a direction (the chunks'; none for many sequences or short ones), for what the forward pass
 // keeps for the backward pass, and for the shares of dB, dC and of the parameters' gradients.
-int64_t esgd_selective_scan_local(const esgd_scan* e) { return local_floats(scan_of(e)); }
+int64_t esgd_selective_scan_local(const esgd_scan* e, int backward) { return local_floats(scan_of(e, backward)); }
 int64_t esgd_selective_scan_keep(const esgd_scan* e) {
   return (e->length + kKeep - 1) / kKeep * e->batch * e->channels * lanes_of(e->states) * kStates;
 }
@@ -900,10 +921,10 @@ int64_t esgd_selective_scan_narrow(const esgd_scan* e) {
   const int side = state_blocks(e->states);
   return blocks_of(e->channels, 32 / side) * e->batch * e->length * 2 * 16 * side;
 }
-int64_t esgd_selective_scan_parts(const esgd_scan* e) { return e->length > 0 ? e->batch * scan_of(e).chunks : 0; }
+int64_t esgd_selective_scan_parts(const esgd_scan* e) { return e->length > 0 ? e->batch * scan_of(e, true).chunks : 0; }
 
 int esgd_selective_scan_fwd(const esgd_scan* e, void* out, float* state_out, float* keep, float* local, void* stream) {
-  Scan s = scan_of(e);
+  Scan s = scan_of(e, false);
   if (!taken(s)) return (int)cudaErrorInvalidValue;
   if (s.batch == 0) return 0;
   place(&s, local);
@@ -914,7 +935,7 @@ int esgd_selective_scan_fwd(const esgd_scan* e, void* out, float* state_out, flo
 // sums [parts][channels * states + 2 * channels].
 int esgd_selective_scan_bwd(const esgd_scan* e, const void* dout, const float* keep, void* du, void* ddelta, void* dz, void* dB, void* dC,
                             float* narrow, float* sums, float* local, void* stream) {
-  Scan s = scan_of(e);
+  Scan s = scan_of(e, true);
   if (!taken(s)) return (int)cudaErrorInvalidValue;
   if (s.batch == 0 || s.length == 0) return 0;
   place(&s, local);
@@ -928,7 +949,7 @@ int esgd_selective_scan_bwd(const esgd_scan* e, const void* dout, const float* k
 }
 
 int esgd_selective_scan_step(const esgd_scan* e, float* state_out, void* out, void* stream) {
-  const Scan s = scan_of(e);
+  const Scan s = scan_of(e, false);
   if (!taken(s) || s.state == nullptr) return (int)cudaErrorInvalidValue;
   if (s.batch == 0) return 0;
   const int is_bf16 = e->is_bf16, lanes = lanes_of(s.states);

@@ -12,7 +12,7 @@ int esgd_causal_conv_bwd(const void* x, int64_t xb, int64_t xt, const void* stat
                          int64_t length, int channels, int taps, int act, void* stream);
 int esgd_causal_conv_step(const void* x, int64_t xb, const void* state, void* state_out, const float* weight, const float* bias, void* y,
                           int is_bf16, int64_t batch, int channels, int taps, int act, void* stream);
-int64_t esgd_selective_scan_local(const esgd_scan* e);
+int64_t esgd_selective_scan_local(const esgd_scan* e, int backward);
 int64_t esgd_selective_scan_keep(const esgd_scan* e);
 int64_t esgd_selective_scan_narrow(const esgd_scan* e);
 int64_t esgd_selective_scan_parts(const esgd_scan* e);
@@ -218,7 +218,7 @@ struct SelectiveScanFn : public Function<SelectiveScanFn> {
     variable_list out = {at::empty(in.u.sizes(), in.u.options())};
     if (want_state) out.push_back(at::empty({e.batch, e.channels, e.states}, in.A.options()));
     if (keep != nullptr) *keep = at::empty({esgd_selective_scan_keep(&e)}, in.A.options());
-    const Tensor local = room(esgd_selective_scan_local(&e), in.A.options());
+    const Tensor local = room(esgd_selective_scan_local(&e, 0), in.A.options());
     ck(esgd_selective_scan_fwd(&e, mut(out[0]), want_state ? fptr(out[1]) : nullptr, keep != nullptr ? fptr(*keep) : nullptr, fptr(local),
                                stream_of(in.u)), "selective_scan");
     return out;
@@ -241,7 +241,7 @@ struct SelectiveScanFn : public Function<SelectiveScanFn> {
     const ParamGrad dA(ctx, "A", need[0], {d, n}, f32), dD(ctx, "D", need[1], {d}, f32), db(ctx, "b", need[2], {d}, f32);
     const int64_t parts = esgd_selective_scan_parts(&e);
     const Tensor narrow = at::empty({esgd_selective_scan_narrow(&e)}, f32), sums = at::empty({parts, d * (n + 2)}, f32);
-    const Tensor local = room(esgd_selective_scan_local(&e), f32);
+    const Tensor local = room(esgd_selective_scan_local(&e, 1), f32);
     ck(esgd_selective_scan_bwd(&e, ptr(dout), fptr(keep), mut(du), mut(ddelta), mut(dz), mut(dB), mut(dC), fptr(narrow), fptr(sums),
                                fptr(local), stream_of(in.u)), "selective_scan backward");
     ck(esgd_sum_parts(fptr(sums), parts, dA.out(), d * n, dA.add(), dD.out(), d, dD.add(), db.out(), d, db.add(), stream_of(in.u)),
