@@ -49,7 +49,7 @@ struct Scan {
   const float* state;                // [batch][channels][states], or null: zero
   int64_t batch, length;
   int channels, states, softplus;
-  int even, even_narrow;             // neighbouring channels (states) are one load: even counts, strides and beginnings
+  int even;                          // neighbouring channels and states are one load: even counts, strides and beginnings
   int chunks;
   int64_t chunk;                     // steps of a chunk, a multiple of kTile
   float *local, *span;               // [chunks][batch][channels][kLanes * 4] and [chunks][batch][channels], with more than one chunk
@@ -89,14 +89,14 @@ template <> struct Two<__nv_bfloat16> {
   }
   __device__ __forceinline__ float2 get() const { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 };
-// The values c and c + 1 of a row, as far as its width goes.
-template <class T> __device__ __forceinline__ void put(T* row, int c, int width, bool even, float x, float y) {
-  if (even && c < width) {
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(row + c) = make_float2(x, y);
-    else *reinterpret_cast<__nv_bfloat162*>(row + c) = __floats2bfloat162_rn(x, y);
-  } else {
-    if (c < width) row[c] = as_type<T>(x);
-    if (c + 1 < width) row[c + 1] = as_type<T>(y);
+// Two neighbouring values of a row, or as many as there are.
+template <class T, bool kEven> __device__ __forceinline__ void put(T* to, int in, float x, float y) {
+  if constexpr (!kEven) {
+    if (in > 0) to[0] = as_type<T>(x);
+    if (in > 1) to[1] = as_type<T>(y);
+  } else if (in > 0) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(x, y);
+    else *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(x, y);
   }
 }
 __device__ __forceinline__ float2 two_of(const float* p, int c, int width) {
@@ -184,8 +184,8 @@ template <class T> struct Cursor {
     tile = tile_ * q.t;
   }
   // `n` steps are left from the thread's first on; `in`: how many of the two values there are.
-  template <int kPairs> __device__ __forceinline__ void fetch(Two<T> (&to)[kPairs], int n, int between, int in, bool even) {
-    if (even) {
+  template <bool kEven, int kPairs> __device__ __forceinline__ void fetch(Two<T> (&to)[kPairs], int n, int between, int in) {
+    if constexpr (kEven) {
 #pragma unroll
       for (int k = 0; k < kPairs; ++k)
         if (k * between < n && in > 0) to[k].load(p + k * pitch);
@@ -228,7 +228,7 @@ template <int kLanes> __device__ __forceinline__ void states_of(const float* p, 
 }
 
 // keep: [tiles of kKeep steps][batch][channels][kLanes * 4], the state ahead of every eighth step; or null.
-template <class T, int kLanes>
+template <class T, int kLanes, bool kEven>
 __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T* __restrict__ out, float* __restrict__ state_out,
                                                                       float* __restrict__ keep) {
   pdl_enter();
@@ -252,11 +252,11 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
   const bool gated = s.z.p != nullptr;
   auto prefetch = [&](int steps) {
     const int n = steps - in.step, m = steps - in.narrow_step;
-    at_u.template fetch<In::kPairs>(u, n, In::kPitch, two, s.even);
-    at_delta.template fetch<In::kPairs>(delta, n, In::kPitch, two, s.even);
-    if (gated) at_z.template fetch<In::kPairs>(z, n, In::kPitch, two, s.even);
-    at_b.template fetch<In::kNarrow>(bb, m, In::kNarrowPitch, narrow_two, s.even_narrow);
-    at_c.template fetch<In::kNarrow>(cc, m, In::kNarrowPitch, narrow_two, s.even_narrow);
+    at_u.template fetch<kEven, In::kPairs>(u, n, In::kPitch, two);
+    at_delta.template fetch<kEven, In::kPairs>(delta, n, In::kPitch, two);
+    if (gated) at_z.template fetch<kEven, In::kPairs>(z, n, In::kPitch, two);
+    at_b.template fetch<kEven, In::kNarrow>(bb, m, In::kNarrowPitch, narrow_two);
+    at_c.template fetch<kEven, In::kNarrow>(cc, m, In::kNarrowPitch, narrow_two);
   };
 #pragma unroll
   for (int k = 0; k < In::kPairs; ++k) u[k] = delta[k] = z[k] = Two<T>{};
@@ -270,7 +270,6 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
   if (s.chunks > 1 && on) joined<kLanes, false>(s, p.b, p.chunk, channel, on, lane, a, h);
   T* y = out + (p.b * s.length + p.first + in.step) * s.channels + p.c0 + in.channel;
   const int64_t y_pitch = (int64_t)In::kPitch * s.channels, kept_tile = s.batch * s.channels * kLanes;
-  const bool even_out = s.channels % 2 == 0;
   float4* kept = keep != nullptr && on > 0
       ? reinterpret_cast<float4*>(keep) + ((p.first / kKeep * s.batch + p.b) * s.channels + channel) * kLanes + lane : nullptr;
   const float2 skip = two_of(s.D, p.c0 + in.channel, s.channels), bias = two_of(s.bias, p.c0 + in.channel, s.channels);
@@ -343,14 +342,14 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
         v += part.x;
         w += part.y;
       }
-      put<T>(y + k * y_pitch, 0, two, even_out, (v + du[k].x) * gate[k].x, (w + du[k].y) * gate[k].y);
+      put<T, kEven>(y + k * y_pitch, two, (v + du[k].x) * gate[k].x, (w + du[k].y) * gate[k].y);
     }
     y += (int64_t)kTile * s.channels;
   }
   // behind the end: the rows of the chunk that are left
   T* rest = out + p.b * s.length * s.channels + p.c0 + in.channel;
   for (int64_t t = (p.first > p.len ? p.first : p.len) + in.step; t < p.end; t += In::kPitch)
-    put<T>(rest + t * s.channels, 0, two, even_out, 0.0f, 0.0f);
+    put<T, kEven>(rest + t * s.channels, two, 0.0f, 0.0f);
   // the chunk that the sequence ends in
   if (state_out != nullptr && (p.first < p.len || p.chunk == 0) && p.end >= p.len)
 #pragma unroll
@@ -363,7 +362,7 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
 }
 
 // A chunk by itself, from a state of zero: forward h, or backward the carry a dh that leaves its first step; and the sum of its dt.
-template <class T, int kLanes, bool kReverse>
+template <class T, int kLanes, bool kReverse, bool kEven>
 __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, const T* __restrict__ dout) {
   pdl_enter();
   using In = Lanes<kLanes>;
@@ -389,13 +388,12 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
   for (int k = 0; k < In::kPairs; ++k) x[k] = delta[k] = z[k] = Two<T>{};
 #pragma unroll
   for (int k = 0; k < In::kNarrow; ++k) bc[k] = Two<T>{};
-  const bool even_x = kReverse ? s.channels % 2 == 0 : s.even != 0;
   auto prefetch = [&](int steps) {
     const int n = steps - in.step, m = steps - in.narrow_step;
-    at_x.template fetch<In::kPairs>(x, n, In::kPitch, two, even_x);
-    at_delta.template fetch<In::kPairs>(delta, n, In::kPitch, two, s.even);
-    if (gated) at_z.template fetch<In::kPairs>(z, n, In::kPitch, two, s.even);
-    at_bc.template fetch<In::kNarrow>(bc, m, In::kNarrowPitch, narrow_two, s.even_narrow);
+    at_x.template fetch<kEven, In::kPairs>(x, n, In::kPitch, two);
+    at_delta.template fetch<kEven, In::kPairs>(delta, n, In::kPitch, two);
+    if (gated) at_z.template fetch<kEven, In::kPairs>(z, n, In::kPitch, two);
+    at_bc.template fetch<kEven, In::kNarrow>(bc, m, In::kNarrowPitch, narrow_two);
   };
   int steps = (int)(p.last - t1 < kTile ? p.last - t1 : kTile);
   if (tiles > 0) prefetch(steps);
@@ -487,12 +485,12 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 // d += a b with eleven bits of each factor, or (fp32 gradients) with the next eleven as well.
-template <bool kFine> __device__ __forceinline__ void product(float (&d)[4], const float (&a)[4], const float (&b)[2]) {
-  uint32_t ah[4], bh[2];
+// bh: the rounded factor.
+template <bool kFine>
+__device__ __forceinline__ void product(float (&d)[4], const float (&a)[4], const uint32_t (&bh)[2], const float (&b)[2]) {
+  uint32_t ah[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) ah[i] = tf32(a[i]);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) bh[i] = tf32(b[i]);
   mma(d, ah, bh);
   if constexpr (kFine) {
     uint32_t al[4], bl[2];
@@ -508,7 +506,7 @@ template <bool kFine> __device__ __forceinline__ void product(float (&d)[4], con
 // A warp: eight channels and sixteen states.  Thread: channels 2 c and 2 c + 1 (c = lane % 4, the fragments' columns c and c + 4),
 // states n and n + 8 (n = lane / 4, their rows).
 // kBlocks warps side by side have the states of wider layers.
-template <class T, int kBlocks>
+template <class T, int kBlocks, bool kEven>
 __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s, Grads g) {
   pdl_enter();
   constexpr int kWarps = kThreads / 32, kWide = 8 * kWarps / kBlocks, kPadded = 16 * kBlocks, kSlots = 8 * kBlocks;
@@ -549,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
   // a thread prepares and finishes two channels of a step, and prepares some of B and C
   const In in;
   const int two = left_of(s.channels, p.c0 + in.channel), narrow_two = left_of(s.states, in.state);
-  const bool mine = in.step < kKeep, gated = s.z.p != nullptr, even = s.channels % 2 == 0;
+  const bool mine = in.step < kKeep, gated = s.z.p != nullptr;
   const float2 skip = two_of(s.D, p.c0 + in.channel, s.channels), bias = two_of(s.bias, p.c0 + in.channel, s.channels);
   float2 dD = make_float2(0.0f, 0.0f), dbias = dD;
   const int64_t tiles = p.first < p.last ? (p.last - p.first + kKeep - 1) / kKeep : 0;
@@ -567,12 +565,12 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
   float kept[2][2];
   auto prefetch = [&](int steps) {
     const int n = mine ? steps - in.step : 0, m = steps - in.narrow_step;
-    at_u.template fetch<1>(u, n, 0, two, s.even);
-    at_delta.template fetch<1>(delta, n, 0, two, s.even);
-    if (gated) at_z.template fetch<1>(z, n, 0, two, s.even);
-    at_up.template fetch<1>(up, n, 0, two, even);
-    at_b.template fetch<In::kNarrow>(bb, m, In::kNarrowPitch, narrow_two, s.even_narrow);
-    at_c.template fetch<In::kNarrow>(cc, m, In::kNarrowPitch, narrow_two, s.even_narrow);
+    at_u.template fetch<kEven, 1>(u, n, 0, two);
+    at_delta.template fetch<kEven, 1>(delta, n, 0, two);
+    if (gated) at_z.template fetch<kEven, 1>(z, n, 0, two);
+    at_up.template fetch<kEven, 1>(up, n, 0, two);
+    at_b.template fetch<kEven, In::kNarrow>(bb, m, In::kNarrowPitch, narrow_two);
+    at_c.template fetch<kEven, In::kNarrow>(cc, m, In::kNarrowPitch, narrow_two);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -637,8 +635,10 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
       }
     }
     // step lane / 4 is the column of the fragments that this lane has
-    const float2 own_dy = halves(s_dy[lane / 4][w0 / 2]);
-    const float2 own_du = halves(reinterpret_cast<const ulonglong2*>(&s_dt[lane / 4][w0 / 2])->y);
+    const float2 column_dy = halves(s_dy[lane / 4][w0 / 2]);
+    const float2 column_du = halves(reinterpret_cast<const ulonglong2*>(&s_dt[lane / 4][w0 / 2])->y);
+    const float own_dy[2] = {column_dy.x, column_dy.y}, own_du[2] = {column_du.x, column_du.y};
+    const uint32_t own_dyh[2] = {tf32(column_dy.x), tf32(column_dy.y)}, own_duh[2] = {tf32(column_du.x), tf32(column_du.y)};
     float dB[4] = {0, 0, 0, 0}, dC[4] = {0, 0, 0, 0};        // state n (n + 8), steps 2 (lane % 4) and the next
     dA[0] = dA[1] = 0;
 #pragma unroll
@@ -657,11 +657,19 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
       *reinterpret_cast<f2*>(&s_part[1][t][slot][w0]) = fma2(dh[1], bc.y, mul2(dh[0], bc.x));
       *reinterpret_cast<f2*>(&s_part[2][t][slot][w0]) = fma2(da[1], A[1], mul2(da[0], A[0]));
       const bool column = lane / 4 == t;
-      const float by[2] = {column ? own_dy.x : 0.0f, column ? own_dy.y : 0.0f}, bu[2] = {column ? own_du.x : 0.0f, column ? own_du.y : 0.0f};
+      float by[2], bu[2];
+      uint32_t byh[2], buh[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        byh[i] = column ? own_dyh[i] : 0u;
+        buh[i] = column ? own_duh[i] : 0u;
+        by[i] = column ? own_dy[i] : 0.0f;          // fp32 gradients alone read them
+        bu[i] = column ? own_du[i] : 0.0f;
+      }
       const float2 h0 = halves(h[t + 1][0]), h1 = halves(h[t + 1][1]), d0 = halves(dh[0]), d1 = halves(dh[1]);
       const float ha[4] = {h0.x, h1.x, h0.y, h1.y}, da4[4] = {d0.x, d1.x, d0.y, d1.y};
-      product<kFine>(dC, ha, by);
-      product<kFine>(dB, da4, bu);
+      product<kFine>(dC, ha, byh, by);
+      product<kFine>(dB, da4, buh, bu);
     }
     // into the running sum with its rounding errors beside it: a sequence has thousands of terms
 #pragma unroll
@@ -704,10 +712,10 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
         }
         v[q] = make_float2(x, w);
       }
-      if (to_dz != nullptr) put<T>(to_dz, 0, two, even, dz.x * fmaf(skip.x, uv.x, v[0].x), dz.y * fmaf(skip.y, uv.y, v[0].y));
-      put<T>(to_du, 0, two, even, fmaf(v[1].x, dt.x, skip.x * dy.x), fmaf(v[1].y, dt.y, skip.y * dy.y));
+      if (to_dz != nullptr) put<T, kEven>(to_dz, two, dz.x * fmaf(skip.x, uv.x, v[0].x), dz.y * fmaf(skip.y, uv.y, v[0].y));
+      put<T, kEven>(to_du, two, fmaf(v[1].x, dt.x, skip.x * dy.x), fmaf(v[1].y, dt.y, skip.y * dy.y));
       const float ex = fmaf(v[1].x, uv.x, v[2].x) * slope_dt.x, ew = fmaf(v[1].y, uv.y, v[2].y) * slope_dt.y;
-      put<T>(to_ddelta, 0, two, even, ex, ew);
+      put<T, kEven>(to_ddelta, two, ex, ew);
       dD.x = fmaf(dy.x, uv.x, dD.x);
       dD.y = fmaf(dy.y, uv.y, dD.y);
       dbias.x += ex;
@@ -721,9 +729,9 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
   const int64_t lead = p.b * s.length * s.channels + p.c0 + in.channel;
   for (int64_t t = (p.first > p.len ? p.first : p.len) + in.step; t < p.end; t += In::kPitch) {
     const int64_t row = lead + t * s.channels;
-    put<T>(reinterpret_cast<T*>(g.du) + row, 0, two, even, 0.0f, 0.0f);
-    put<T>(reinterpret_cast<T*>(g.ddelta) + row, 0, two, even, 0.0f, 0.0f);
-    if (g.dz != nullptr) put<T>(reinterpret_cast<T*>(g.dz) + row, 0, two, even, 0.0f, 0.0f);
+    put<T, kEven>(reinterpret_cast<T*>(g.du) + row, two, 0.0f, 0.0f);
+    put<T, kEven>(reinterpret_cast<T*>(g.ddelta) + row, two, 0.0f, 0.0f);
+    if (g.dz != nullptr) put<T, kEven>(reinterpret_cast<T*>(g.dz) + row, two, 0.0f, 0.0f);
   }
   float* sums = g.sums + (p.b * s.chunks + p.chunk) * (int64_t)s.channels * (s.states + 2);
 #pragma unroll
@@ -742,8 +750,8 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
       v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
     }
     float* to = sums + (int64_t)s.channels * s.states;
-    put<float>(to + p.c0 + in.channel, 0, two, false, v.x, v.y);
-    put<float>(to + s.channels + p.c0 + in.channel, 0, two, false, v.z, v.w);
+    put<float, false>(to + p.c0 + in.channel, two, v.x, v.y);
+    put<float, false>(to + s.channels + p.c0 + in.channel, two, v.z, v.w);
   }
 }
 
@@ -803,7 +811,7 @@ __global__ void __launch_bounds__(kThreads) selective_scan_step_kernel(Scan s, f
 }
 
 int lanes_of(int states) {
-  int l = 1;
+  int l = 2;
   while (l * kStates < states) l *= 2;
   return l;
 }
@@ -835,28 +843,34 @@ void split(Scan* s, int64_t blocks, const Pace& p) {
   }
 }
 
-template <class T, int kLanes> int forward(const Scan& s, void* out, float* state_out, float* keep, void* stream) {
+template <class T, int kLanes, bool kEven> int forward_even(const Scan& s, void* out, float* state_out, float* keep, void* stream) {
   static SmemAllowed allowed{0};
   constexpr int kWide = Lanes<kLanes>::kWide;
   constexpr size_t kSmem = kTile * (2 * kLanes * 16 + kWide * 8 + kLanes * Lanes<kLanes>::kRow * 4);
   if (kSmem > 48 * 1024) {
-    const int rc = allow_smem(selective_scan_fwd_kernel<T, kLanes>, kSmem, allowed);
+    const int rc = allow_smem(selective_scan_fwd_kernel<T, kLanes, kEven>, kSmem, allowed);
     if (rc != 0) return rc;
   }
   const dim3 grid((unsigned)(s.batch * s.chunks * blocks_of(s.channels, kWide)));
   if (s.chunks > 1) {
-    const int rc = launch(selective_scan_chunk_kernel<T, kLanes, false>, grid, kThreads, 0, stream, s, (const T*)nullptr);
+    const int rc = launch(selective_scan_chunk_kernel<T, kLanes, false, kEven>, grid, kThreads, 0, stream, s, (const T*)nullptr);
     if (rc != 0) return rc;
   }
-  return launch(selective_scan_fwd_kernel<T, kLanes>, grid, kThreads, kSmem, stream, s, (T*)out, state_out, keep);
+  return launch(selective_scan_fwd_kernel<T, kLanes, kEven>, grid, kThreads, kSmem, stream, s, (T*)out, state_out, keep);
+}
+template <class T, int kLanes> int forward(const Scan& s, void* out, float* state_out, float* keep, void* stream) {
+  return s.even ? forward_even<T, kLanes, true>(s, out, state_out, keep, stream) : forward_even<T, kLanes, false>(s, out, state_out, keep, stream);
 }
 template <class T, int kLanes> int carries(const Scan& s, const void* dout, void* stream) {
   const dim3 grid((unsigned)(s.batch * s.chunks * blocks_of(s.channels, Lanes<kLanes>::kWide)));
-  return launch(selective_scan_chunk_kernel<T, kLanes, true>, grid, kThreads, 0, stream, s, (const T*)dout);
+  return s.even ? launch(selective_scan_chunk_kernel<T, kLanes, true, true>, grid, kThreads, 0, stream, s, (const T*)dout)
+                : launch(selective_scan_chunk_kernel<T, kLanes, true, false>, grid, kThreads, 0, stream, s, (const T*)dout);
 }
 template <class T, int kBlocks> int backward_blocks(const Scan& s, const Grads& g, void* dB, void* dC, void* stream) {
   const int blocks = blocks_of(s.channels, 32 / kBlocks), padded = 16 * kBlocks;
-  const int rc = launch(selective_scan_bwd_kernel<T, kBlocks>, dim3((unsigned)(s.batch * s.chunks * blocks)), kThreads, 0, stream, s, g);
+  const dim3 grid((unsigned)(s.batch * s.chunks * blocks));
+  const int rc = s.even ? launch(selective_scan_bwd_kernel<T, kBlocks, true>, grid, kThreads, 0, stream, s, g)
+                        : launch(selective_scan_bwd_kernel<T, kBlocks, false>, grid, kThreads, 0, stream, s, g);
   if (rc != 0) return rc;
   const int64_t n = s.batch * s.length * 2 * padded;
   return launch(selective_scan_narrow_kernel<T>, dim3((unsigned)((n + 255) / 256)), 256, 0, stream, g.narrow, blocks, s, padded, (T*)dB, (T*)dC);
@@ -875,8 +889,7 @@ template <class T, int kLanes> int step(const Scan& s, float* state_out, void* o
 
 // F<T, kLanes>(...)
 #define ESGD_LANES(T, F, ...)                                                                                   \
-  (lanes == 1 ? F<T, 1>(__VA_ARGS__) : lanes == 2 ? F<T, 2>(__VA_ARGS__) : lanes == 4 ? F<T, 4>(__VA_ARGS__)    \
-   : lanes == 8 ? F<T, 8>(__VA_ARGS__) : F<T, 16>(__VA_ARGS__))
+  (lanes == 2 ? F<T, 2>(__VA_ARGS__) : lanes == 4 ? F<T, 4>(__VA_ARGS__) : lanes == 8 ? F<T, 8>(__VA_ARGS__) : F<T, 16>(__VA_ARGS__))
 #define ESGD_TYPE(F, ...) (is_bf16 ? ESGD_LANES(__nv_bfloat16, F, __VA_ARGS__) : ESGD_LANES(float, F, __VA_ARGS__))
 
 bool taken(const Scan& s) { return s.states >= 1 && s.states <= 64 && s.channels >= 1 && s.batch >= 0 && s.length >= 0; }
@@ -885,11 +898,10 @@ Scan scan_of(const esgd_scan* e, bool backward) {
   Scan s = {};
   Seq* q[5] = {&s.u, &s.delta, &s.z, &s.B, &s.C};
   const uintptr_t size = e->is_bf16 ? 2 : 4;
-  s.even = e->channels % 2 == 0;
-  s.even_narrow = e->states % 2 == 0;
+  s.even = e->channels % 2 == 0 && e->states % 2 == 0;
   for (int i = 0; i < 5; ++i) {
     *q[i] = {e->p[i], e->b[i], e->t[i]};
-    if (e->p[i] != nullptr && ((uintptr_t)e->p[i] % (2 * size) || e->b[i] % 2 || e->t[i] % 2)) (i < 3 ? s.even : s.even_narrow) = 0;
+    if (e->p[i] != nullptr && ((uintptr_t)e->p[i] % (2 * size) || e->b[i] % 2 || e->t[i] % 2)) s.even = 0;
   }
   s.A = e->A; s.D = e->D; s.bias = e->bias;
   s.lengths = e->lengths;
