@@ -92,6 +92,85 @@ template <int kAct> __device__ __forceinline__ float slope(float x) {
   }
 }
 
+// Paired fp32 arithmetic: two values in a 64-bit register, one instruction for both.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ f2 pair(float2 v) { return pair(v.x, v.y); }
+__device__ __forceinline__ float2 halves(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// Both halves by one factor.
+__device__ __forceinline__ f2 mul2(f2 a, float b) {
+  const float2 v = halves(a);
+  return pair(v.x * b, v.y * b);
+}
+__device__ __forceinline__ f2 fma2(f2 a, float b, f2 c) {
+  const float2 v = halves(a), w = halves(c);
+  return pair(fmaf(v.x, b, w.x), fmaf(v.y, b, w.y));
+}
+__device__ __forceinline__ f2 exp2_2(f2 x) {
+  const float2 v = halves(x);
+  return pair(exp2_approx(v.x), exp2_approx(v.y));
+}
+__device__ __forceinline__ f2 sigmoid2(f2 x) {
+  const float2 v = halves(add2(exp2_2(mul2(x, pair(-kLog2e, -kLog2e))), pair(1.0f, 1.0f)));
+  return pair(reciprocal(v.x), reciprocal(v.y));
+}
+template <int kAct> __device__ __forceinline__ f2 activate2(f2 x) {
+  if constexpr (kAct == kActSilu) {
+    return mul2(x, sigmoid2(x));
+  } else if constexpr (kAct == kActRelu) {
+    const float2 v = halves(x);
+    return pair(activate<kActRelu>(v.x), activate<kActRelu>(v.y));
+  } else {
+    return x;
+  }
+}
+template <int kAct> __device__ __forceinline__ f2 slope2(f2 x) {
+  if constexpr (kAct == kActSilu) {
+    const f2 s = sigmoid2(x), xs = mul2(x, s);
+    return add2(fma2(mul2(xs, pair(-1.0f, -1.0f)), s, xs), s);      // s + x s (1 - s)
+  } else {
+    const float2 v = halves(x);
+    return pair(slope<kAct>(v.x), slope<kAct>(v.y));
+  }
+}
+// A vector as pairs (a single element: a pair with a zero).
+template <int kV> struct PairsOf { static constexpr int n = (kV + 1) / 2; };
+template <class T, int kV> __device__ __forceinline__ void unpack2(const Pack<T, kV>& r, f2 (&f)[PairsOf<kV>::n]) {
+  float v[kV];
+  unpack<T, kV>(r, v);
+#pragma unroll
+  for (int q = 0; q < PairsOf<kV>::n; ++q) f[q] = pair(v[2 * q], 2 * q + 1 < kV ? v[(2 * q + 1) % kV] : 0.0f);
+}
+template <class T, int kV> __device__ __forceinline__ void store2(T* p, const f2 (&f)[PairsOf<kV>::n]) {
+  float v[kV];
+#pragma unroll
+  for (int q = 0; q < kV; ++q) v[q] = q % 2 == 0 ? halves(f[q / 2]).x : halves(f[q / 2]).y;
+  store<T, kV>(p, v);
+}
+
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace esgd

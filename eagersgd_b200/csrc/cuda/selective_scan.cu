@@ -103,43 +103,6 @@ __device__ __forceinline__ float2 two_of(const float* p, int c, int width) {
   return make_float2(p != nullptr && c < width ? p[c] : 0.0f, p != nullptr && c + 1 < width ? p[c + 1] : 0.0f);
 }
 
-// Paired fp32 arithmetic.
-using f2 = unsigned long long;
-__device__ __forceinline__ f2 pair(float a, float b) {
-  f2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 halves(f2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-  f2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-  f2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f2 exp2_2(f2 x) {
-  const float2 v = halves(x);
-  return pair(exp2_approx(v.x), exp2_approx(v.y));
-}
-__device__ __forceinline__ f2 pair(float2 v) { return pair(v.x, v.y); }
-// Both halves by one factor.
-__device__ __forceinline__ f2 mul2(f2 a, float b) {
-  const float2 v = halves(a);
-  return pair(v.x * b, v.y * b);
-}
-__device__ __forceinline__ f2 fma2(f2 a, float b, f2 c) {
-  const float2 v = halves(a), w = halves(c);
-  return pair(fmaf(v.x, b, w.x), fmaf(v.y, b, w.y));
-}
-
 // A block: a sequence's channels [c0, c0 + kWide) and steps [first, last) of a chunk, as far as the sequence goes.
 template <int kWide_> struct Block {
   static constexpr int kWide = kWide_;

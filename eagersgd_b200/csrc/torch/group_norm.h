@@ -125,7 +125,8 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const Tensor& gamma, cons
   TORCH_CHECK(c / groups <= esgd_group_norm_max_group(), "group_norm_act: takes up to ", esgd_group_norm_max_group(), " channels a group, not ",
               c / groups);
   TORCH_CHECK(act >= 0 && act <= 2 && eps >= 0, "group_norm_act: no such activation, or an eps below zero");
-  TORCH_CHECK(c < ((int64_t)1 << 31) && x.size(0) * c < ((int64_t)1 << 27), "group_norm_act: an input of ", x.sizes(), " is too large");
+  TORCH_CHECK(c < ((int64_t)1 << 31) && x.size(0) * c < ((int64_t)1 << 27) && x.size(2) * x.size(3) < ((int64_t)1 << 30),
+              "group_norm_act: an input of ", x.sizes(), " is too large");
   check_vector("group_norm_act", "gamma", gamma, x, c);
   check_vector("group_norm_act", "beta", beta, x, c);
   if (res.has_value()) {
