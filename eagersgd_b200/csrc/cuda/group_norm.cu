@@ -34,6 +34,9 @@ struct Shape {
   float eps;
 };
 
+// The backward pass' sums of two sets, and later three rows of coefficients.
+__host__ __device__ constexpr int stage_floats(int v, int slice) { return 2 * kThreads * v > 3 * slice ? 2 * kThreads * v : (3 * slice + 3) / 4 * 4; }
+
 // Where a thread works: a vector of kV channels, every `lanes`-th row of its CTA's.
 template <int kV> struct Place {
   int vectors, wide, lanes, lane, vec;
@@ -58,75 +61,123 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sums over the CTA's rows of the threads' channels, into out[channel * stride] from channel v0 * kV on.  Every thread calls it.
-template <int kV>
-__device__ __forceinline__ void channel_sums(const Place<kV>& p, const f2 (&pairs)[PairsOf<kV>::n], int v0, float* stage, float* out, int stride) {
-  int partial = p.lanes;
-  float a[kV];
+// Sums over the CTA's rows of the threads' channels (kSets of them at a time), into out[set * slice + channel] from channel v0 * kV
+// on.  Every thread calls it.
+template <int kSets, int kV>
+__device__ __forceinline__ void channel_sums(const Place<kV>& p, const f2 (&sets)[kSets][PairsOf<kV>::n], int v0, float* stage, float* out, int slice) {
+  int partial = p.lanes, row = p.lane;
+  bool writes = p.lane < p.lanes;
+  float a[kSets][kV];
 #pragma unroll
-  for (int q = 0; q < kV; ++q) a[q] = q % 2 == 0 ? halves(pairs[q / 2]).x : halves(pairs[q / 2]).y;
+  for (int i = 0; i < kSets; ++i)
+#pragma unroll
+    for (int q = 0; q < kV; ++q) a[i][q] = q % 2 == 0 ? halves(sets[i][q / 2]).x : halves(sets[i][q / 2]).y;
   if (p.fold) {
     partial = kThreads / 32;
+    row = threadIdx.x / 32;
+    writes = (threadIdx.x & 31) < p.wide;
     for (int o = p.wide; o < 32; o *= 2)
 #pragma unroll
-      for (int q = 0; q < kV; ++q) a[q] += __shfl_xor_sync(0xffffffffu, a[q], o);
-    if ((threadIdx.x & 31) < p.wide)
+      for (int i = 0; i < kSets; ++i)
 #pragma unroll
-      for (int q = 0; q < kV; ++q) stage[(threadIdx.x / 32 * p.wide + p.vec) * kV + q] = a[q];
-  } else if (p.lane < p.lanes) {
-#pragma unroll
-    for (int q = 0; q < kV; ++q) stage[threadIdx.x * kV + q] = a[q];
+        for (int q = 0; q < kV; ++q) a[i][q] += __shfl_xor_sync(0xffffffffu, a[i][q], o);
   }
+  const int pitch = p.wide * kV;
+  if (writes)
+#pragma unroll
+    for (int i = 0; i < kSets; ++i)
+#pragma unroll
+      for (int q = 0; q < kV; ++q) stage[(i * partial + row) * pitch + p.vec * kV + q] = a[i][q];
   __syncthreads();
   const int here = min(p.wide, p.vectors - v0) * kV;
-  for (int c = threadIdx.x; c < here; c += kThreads) {
+  for (int c = threadIdx.x; c < kSets * here; c += kThreads) {
+    const int i = kSets > 1 && c >= here ? 1 : 0, ch = c - i * here;
     float t = 0.0f;
-    for (int r = 0; r < partial; ++r) t += stage[r * p.wide * kV + c];
-    out[(v0 * kV + c) * stride] = t;
+    for (int r = 0; r < partial; ++r) t += stage[(i * partial + r) * pitch + ch];
+    out[i * slice + v0 * kV + ch] = t;
   }
   __syncthreads();
 }
+// A thread's channels of a row of shared memory.
+template <int kV> __device__ __forceinline__ void channels_of(const float* p, f2 (&to)[PairsOf<kV>::n]) {
+  if constexpr (kV == 1) {
+    to[0] = pair(p[0], 0.0f);
+  } else {
+#pragma unroll
+    for (int q = 0; q < kV / 4; ++q) {
+      const float4 v = *reinterpret_cast<const float4*>(p + 4 * q);
+      to[2 * q] = pair(v.x, v.y);
+      to[2 * q + 1] = pair(v.z, v.w);
+    }
+  }
+}
 
-// Rows of one tensor: the first `held` of a CTA in shared memory, each thread's own vectors, the others where they are.
-template <class T, int kV> struct Rows {
-  const T* p;          // the CTA's first row and the slice's first channel
-  T* in;               // [held][slice]
+// Rows of kMany tensors from `base` on: the first `held` of a CTA in shared memory, each thread's own vectors, the others where they
+// are.
+template <class T, int kV, int kMany> struct Rows {
+  const T* p[kMany];   // the CTA's first row and the slice's first channel
+  T* in;               // [kMany][held][slice]
   int held, slice;
   int64_t pitch;
-  __device__ Rows(const T* p_, T* in_, const Shape& s) : p(p_), in(in_), held(s.held), slice(s.slice), pitch(s.channels) {}
+  __device__ Rows(T* in_, const Shape& s) : in(in_), held(s.held), slice(s.slice), pitch(s.channels) {}
   __device__ __forceinline__ void ask(const Place<kV>& pl) const {
     if constexpr (kV > 1) {
       const int n = held < pl.rows ? held : pl.rows;
-      for (int v = pl.vec; pl.on(v); v += pl.wide) {
-        const T* from = p + pl.lane * pitch + v * kV;
-        uint32_t to = (uint32_t)__cvta_generic_to_shared(in + pl.lane * slice + v * kV);
-        for (int r = pl.lane; r < n; r += pl.lanes) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-          from += pl.lanes * pitch;
-          to += pl.lanes * slice * (int)sizeof(T);
+      for (int v = pl.vec; pl.on(v); v += pl.wide)
+#pragma unroll
+        for (int i = 0; i < kMany; ++i) {
+          const T* from = p[i] + pl.lane * pitch + v * kV;
+          uint32_t to = (uint32_t)__cvta_generic_to_shared(in + (i * held + pl.lane) * slice + v * kV);
+          for (int r = pl.lane; r < n; r += pl.lanes) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+            from += pl.lanes * pitch;
+            to += pl.lanes * slice * (int)sizeof(T);
+          }
         }
-      }
     }
   }
-  __device__ __forceinline__ Pack<T, kV> row(int r, int v) const {
-    if (kV > 1 && r < held) return load<T, kV>(in + r * slice + v * kV);
-    return load<T, kV>(p + r * pitch + v * kV);
+  // use(vectors, the vector of `more`, their offset from p[]) for a thread's rows; kAhead of them are loaded at a time.
+  template <int kAhead, bool kMore, class Use> __device__ __forceinline__ void each(const Place<kV>& pl, int v, const T* more, Use use) const {
+    const int lanes = pl.lanes, n = kV == 1 ? 0 : held < pl.rows ? held : pl.rows, next = lanes * slice;
+    const int64_t down = lanes * pitch;
+    const T* own = in + pl.lane * slice + v * kV;
+    int64_t o = pl.lane * pitch + v * kV;
+    int r = pl.lane;
+    Pack<T, kV> x[kAhead][kMany], e[kAhead];
+    for (; r + (kAhead - 1) * lanes < n; r += kAhead * lanes, o += kAhead * down, own += kAhead * next) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if constexpr (kMore) e[u] = load<T, kV>(more + o + u * down);
+#pragma unroll
+        for (int i = 0; i < kMany; ++i) x[u][i] = load<T, kV>(own + i * held * slice + u * next);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) use(x[u], e[u], o + u * down);
+    }
+    for (; r < n; r += lanes, o += down, own += next) {
+      if constexpr (kMore) e[0] = load<T, kV>(more + o);
+#pragma unroll
+      for (int i = 0; i < kMany; ++i) x[0][i] = load<T, kV>(own + i * held * slice);
+      use(x[0], e[0], o);
+    }
+    for (; r + (kAhead - 1) * lanes < pl.rows; r += kAhead * lanes, o += kAhead * down) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if constexpr (kMore) e[u] = load<T, kV>(more + o + u * down);
+#pragma unroll
+        for (int i = 0; i < kMany; ++i) x[u][i] = load<T, kV>(p[i] + o + u * down);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) use(x[u], e[u], o + u * down);
+    }
+    for (; r < pl.rows; r += lanes, o += down) {
+      if constexpr (kMore) e[0] = load<T, kV>(more + o);
+#pragma unroll
+      for (int i = 0; i < kMany; ++i) x[0][i] = load<T, kV>(p[i] + o);
+      use(x[0], e[0], o);
+    }
   }
 };
-// f(row, of which u-th of kMany at a time): loads first, then what is done with them.
-template <int kMany, class Load, class Use> __device__ __forceinline__ void over_rows(int first, int step, int rows, Load load_row, Use use_row) {
-  int r = first;
-  for (; r + (kMany - 1) * step < rows; r += kMany * step) {
-#pragma unroll
-    for (int u = 0; u < kMany; ++u) load_row(r + u * step, u);
-#pragma unroll
-    for (int u = 0; u < kMany; ++u) use_row(r + u * step, u);
-  }
-  for (; r < rows; r += step) {
-    load_row(r, 0);
-    use_row(r, 0);
-  }
-}
 __device__ __forceinline__ void arrived() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // The unit that a cluster works on.
@@ -143,7 +194,7 @@ struct Unit {
 };
 
 template <class T, int kV, int kAct, bool kAdd>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, 4)
 group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ z, const float* __restrict__ gamma,
                       const float* __restrict__ beta, float* __restrict__ stats, Shape s) {
   pdl_enter();
@@ -151,16 +202,16 @@ group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T
   const int groups = s.slice / s.per;
   T* held = reinterpret_cast<T*>(smem4);                   // [held][slice]
   float* stage = reinterpret_cast<float*>(held + s.held * s.slice);
-  float* mean = stage + kThreads * kV;                     // [slice]
-  float* m2 = mean + s.slice;
-  float* gmean = m2 + s.slice;                             // [groups] of this CTA's rows
+  float* mean = stage + kThreads * kV;                     // [slice] the channels' sums, then -means
+  float* m2 = mean + s.slice;                              // [slice], then what a deviation is multiplied with
+  float* shift = m2 + s.slice;                             // [slice]
+  float* gmean = shift + s.slice;                          // [groups] of this CTA's rows
   float* gm2 = gmean + groups;
-  float* scale = gm2 + groups;                             // [groups] of the sample: 1 / deviation, mean
-  float* centre = scale + groups;
   cg::cluster_group cluster = cg::this_cluster();
   const Unit unit(s, s.split > 1 ? (int)cluster.block_rank() : 0);
   const Place<kV> p(s, unit.rank);
-  const Rows<T, kV> in(x + unit.base, held, s);
+  Rows<T, kV, 1> in(held, s);
+  in.p[0] = x + unit.base;
   constexpr int kP = PairsOf<kV>::n;
   const int rows = p.rows;
   in.ask(p);
@@ -168,35 +219,34 @@ group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T
   const float inv_rows = rows > 0 ? 1.0f / (float)rows : 0.0f;
   for (int v0 = 0; v0 < p.vectors; v0 += p.wide) {
     const int v = v0 + p.vec;
-    f2 a[kP] = {};
-    Pack<T, kV> raw[4];
+    f2 a[1][kP] = {};
     if (p.on(v))
-      over_rows<4>(p.lane, p.lanes, rows, [&](int r, int u) { raw[u] = in.row(r, v); }, [&](int, int u) {
+      in.template each<2, false>(p, v, nullptr, [&](const Pack<T, kV>(&raw)[1], const Pack<T, kV>&, int64_t) {
         f2 f[kP];
-        unpack2<T, kV>(raw[u], f);
+        unpack2<T, kV>(raw[0], f);
 #pragma unroll
-        for (int q = 0; q < kP; ++q) a[q] = add2(a[q], f[q]);
+        for (int q = 0; q < kP; ++q) a[0][q] = add2(a[0][q], f[q]);
       });
-    channel_sums<kV>(p, a, v0, stage, mean, 1);
+    channel_sums<1, kV>(p, a, v0, stage, mean, s.slice);
   }
   for (int v0 = 0; v0 < p.vectors; v0 += p.wide) {
     const int v = v0 + p.vec;
-    f2 a[kP] = {}, m[kP];
-    Pack<T, kV> raw[4];
+    f2 a[1][kP] = {}, m[kP];
     if (p.on(v)) {
+      channels_of<kV>(mean + v * kV, m);
 #pragma unroll
-      for (int q = 0; q < kP; ++q) m[q] = pair(-mean[v * kV + 2 * q] * inv_rows, kV > 1 ? -mean[v * kV + 2 * q + 1] * inv_rows : 0.0f);
-      over_rows<4>(p.lane, p.lanes, rows, [&](int r, int u) { raw[u] = in.row(r, v); }, [&](int, int u) {
+      for (int q = 0; q < kP; ++q) m[q] = mul2(m[q], -inv_rows);
+      in.template each<2, false>(p, v, nullptr, [&](const Pack<T, kV>(&raw)[1], const Pack<T, kV>&, int64_t) {
         f2 f[kP];
-        unpack2<T, kV>(raw[u], f);
+        unpack2<T, kV>(raw[0], f);
 #pragma unroll
         for (int q = 0; q < kP; ++q) {
           const f2 d = add2(f[q], m[q]);
-          a[q] = fma2(d, d, a[q]);
+          a[0][q] = fma2(d, d, a[0][q]);
         }
       });
     }
-    channel_sums<kV>(p, a, v0, stage, m2, 1);
+    channel_sums<1, kV>(p, a, v0, stage, m2, s.slice);
   }
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   for (int g = warp; g < groups; g += kThreads / 32) {
@@ -212,10 +262,13 @@ group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T
     if (lane == 0) { gmean[g] = m; gm2[g] = q; }
   }
   if (s.split > 1) cluster.sync(); else __syncthreads();
-  for (int g = threadIdx.x; g < groups; g += kThreads) {
-    float m = 0.0f, q = 0.0f;
+  // every channel's thread joins its group's statistics of all CTAs
+  for (int c = threadIdx.x; c < s.slice; c += kThreads) {
+    const int g = c / s.per;
+    float m = gmean[g], q = gm2[g];
     if (s.split > 1) {
       float part[8];
+      m = q = 0.0f;
 #pragma unroll
       for (int r = 0; r < 8; ++r)
         if (r < s.split) {
@@ -229,55 +282,38 @@ group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T
           const float n = (float)(s.rows * (r + 1) / s.split - s.rows * r / s.split) * (float)s.per, d = part[r] - m;
           q += cluster.map_shared_rank(gm2, r)[g] + n * d * d;
         }
-    } else {
-      m = gmean[g];
-      q = gm2[g];
     }
     const float rstd = rsqrtf(q / ((float)s.rows * (float)s.per) + s.eps);
-    scale[g] = rstd;
-    centre[g] = m;
-    if (unit.rank == 0 && stats != nullptr) {
+    if (unit.rank == 0 && stats != nullptr && c == g * s.per) {
       const int64_t at = unit.sample * (s.channels / s.per) + unit.c0 / s.per + g;
       stats[2 * at] = m;
       stats[2 * at + 1] = rstd;
     }
+    mean[c] = -m;
+    m2[c] = rstd * gamma[unit.c0 + c];
+    shift[c] = beta[unit.c0 + c];
   }
+  if (s.split > 1) cluster.barrier_arrive();      // done with the others' sums
   __syncthreads();
   for (int v = p.vec; p.on(v); v += p.wide) {
     f2 m[kP], k[kP], b[kP];
-    float f[3][kV];
-#pragma unroll
-    for (int q = 0; q < kV; ++q) {
-      const int c = v * kV + q, g = c / s.per;
-      f[0][q] = -centre[g];
-      f[1][q] = scale[g] * gamma[unit.c0 + c];
-      f[2][q] = beta[unit.c0 + c];
-    }
-#pragma unroll
-    for (int q = 0; q < kP; ++q) {
-      m[q] = pair(f[0][2 * q], f[0][(2 * q + 1) % kV]);
-      k[q] = pair(f[1][2 * q], f[1][(2 * q + 1) % kV]);
-      b[q] = pair(f[2][2 * q], f[2][(2 * q + 1) % kV]);
-    }
-    const int64_t at = unit.base + v * kV;
-    Pack<T, kV> raw[4], add[4];
-    over_rows<4>(p.lane, p.lanes, rows, [&](int r, int u) {
-      if constexpr (kAdd) add[u] = load<T, kV>(residual + at + r * in.pitch);
-      raw[u] = in.row(r, v);
-    }, [&](int r, int u) {
+    channels_of<kV>(mean + v * kV, m);
+    channels_of<kV>(m2 + v * kV, k);
+    channels_of<kV>(shift + v * kV, b);
+    in.template each<2, kAdd>(p, v, residual + unit.base, [&](const Pack<T, kV>(&raw)[1], const Pack<T, kV>& more, int64_t o) {
       f2 f[kP], e[kP];
-      unpack2<T, kV>(raw[u], f);
-      if constexpr (kAdd) unpack2<T, kV>(add[u], e);
+      unpack2<T, kV>(raw[0], f);
+      if constexpr (kAdd) unpack2<T, kV>(more, e);
 #pragma unroll
       for (int q = 0; q < kP; ++q) {
         f2 pre = fma2(add2(f[q], m[q]), k[q], b[q]);
         if constexpr (kAdd) pre = add2(pre, e[q]);
         f[q] = activate2<kAct>(pre);
       }
-      store2<T, kV>(z + at + r * in.pitch, f);
+      store2<T, kV>(z + unit.base + o, f);
     });
   }
-  if (s.split > 1) cluster.sync();       // nobody leaves while its sums are being read
+  if (s.split > 1) cluster.barrier_wait();        // nobody leaves while its sums are being read
 }
 
 // sums [samples][2][C]: what a sample adds to dbeta and dgamma.
@@ -291,45 +327,41 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
   const int groups = s.slice / s.per;
   T* held = reinterpret_cast<T*>(smem4);                   // [2][held][slice]: x, dz
   float* stage = reinterpret_cast<float*>(held + 2 * s.held * s.slice);
-  float* own = stage + kThreads * kV;                      // [slice][2] over this CTA's rows
-  float* all = own + 2 * s.slice;                          // [slice][2] over the sample's
-  float* avg = all + 2 * s.slice;                          // [groups][2]
+  float* own = stage + stage_floats(kV, s.slice);          // [2][slice] over this CTA's rows: sum d, sum d n
+  float* coef = own + 2 * s.slice;                         // [4][slice]: 1 / deviation, -mean, gamma, beta; then for dx
+  float* avg = coef + 4 * s.slice;                         // [groups][2]
   cg::cluster_group cluster = cg::this_cluster();
   const Unit unit(s, s.split > 1 ? (int)cluster.block_rank() : 0);
   const Place<kV> p(s, unit.rank);
-  const Rows<T, kV> in(x + unit.base, held, s), up(dz + unit.base, held + s.held * s.slice, s);
+  Rows<T, kV, 2> in(held, s);
+  in.p[0] = x + unit.base;
+  in.p[1] = dz + unit.base;
   constexpr int kP = PairsOf<kV>::n;
   constexpr bool kRead = kAdd && kAct != kActNone;         // the residual moves the activation's slope
-  const int rows = p.rows;
   in.ask(p);
-  up.ask(p);
   const float* st = stats + 2 * (unit.sample * (s.channels / s.per) + unit.c0 / s.per);
+  for (int c = threadIdx.x; c < s.slice; c += kThreads) {
+    const int g = c / s.per;
+    coef[c] = st[2 * g + 1];
+    coef[s.slice + c] = -st[2 * g];
+    coef[2 * s.slice + c] = gamma[unit.c0 + c];
+    coef[3 * s.slice + c] = beta[unit.c0 + c];
+  }
+  __syncthreads();
   // n = (f + c) r, pre = n k + h (+ residual): of a thread's channels
   f2 r_[kP], c_[kP], k[kP], h[kP];
   auto coefficients = [&](int v) {
-    float f[4][kV];
-#pragma unroll
-    for (int q = 0; q < kV; ++q) {
-      const int c = v * kV + q, g = c / s.per;
-      f[0][q] = st[2 * g + 1];
-      f[1][q] = -st[2 * g];
-      f[2][q] = gamma[unit.c0 + c];
-      f[3][q] = beta[unit.c0 + c];
-    }
-#pragma unroll
-    for (int q = 0; q < kP; ++q) {
-      r_[q] = pair(f[0][2 * q], f[0][(2 * q + 1) % kV]);
-      c_[q] = pair(f[1][2 * q], f[1][(2 * q + 1) % kV]);
-      k[q] = pair(f[2][2 * q], f[2][(2 * q + 1) % kV]);
-      h[q] = pair(f[3][2 * q], f[3][(2 * q + 1) % kV]);
-    }
+    channels_of<kV>(coef + v * kV, r_);
+    channels_of<kV>(coef + s.slice + v * kV, c_);
+    channels_of<kV>(coef + 2 * s.slice + v * kV, k);
+    channels_of<kV>(coef + 3 * s.slice + v * kV, h);
   };
   // f: n; d: dz act'(.)
-  auto derive = [&](const Pack<T, kV>& rx, const Pack<T, kV>& rd, const Pack<T, kV>& rr, f2 (&f)[kP], f2 (&d)[kP]) {
+  auto derive = [&](const Pack<T, kV>(&raw)[2], const Pack<T, kV>& more, f2 (&f)[kP], f2 (&d)[kP]) {
     f2 e[kP];
-    unpack2<T, kV>(rx, f);
-    unpack2<T, kV>(rd, d);
-    if constexpr (kRead) unpack2<T, kV>(rr, e);
+    unpack2<T, kV>(raw[0], f);
+    unpack2<T, kV>(raw[1], d);
+    if constexpr (kRead) unpack2<T, kV>(more, e);
 #pragma unroll
     for (int q = 0; q < kP; ++q) {
       f[q] = mul2(add2(f[q], c_[q]), r_[q]);
@@ -342,87 +374,83 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
   };
   if (p.on(p.vec)) coefficients(p.vec);
   arrived();
-  Pack<T, kV> rx[2], rd[2], rr[2];
   for (int v0 = 0; v0 < p.vectors; v0 += p.wide) {
     const int v = v0 + p.vec;
-    f2 a[kP] = {}, b[kP] = {};
+    f2 a[2][kP] = {};
     if (p.on(v)) {
       if (v0 > 0) coefficients(v);
-      const T* more = residual + unit.base + v * kV;
-      over_rows<2>(p.lane, p.lanes, rows, [&](int r, int u) {
-        if constexpr (kRead) rr[u] = load<T, kV>(more + r * in.pitch);
-        rx[u] = in.row(r, v);
-        rd[u] = up.row(r, v);
-      }, [&](int, int u) {
+      in.template each<2, kRead>(p, v, residual + unit.base, [&](const Pack<T, kV>(&raw)[2], const Pack<T, kV>& more, int64_t) {
         f2 f[kP], d[kP];
-        derive(rx[u], rd[u], rr[u], f, d);
+        derive(raw, more, f, d);
 #pragma unroll
-        for (int q = 0; q < kP; ++q) { a[q] = add2(a[q], d[q]); b[q] = fma2(d[q], f[q], b[q]); }
+        for (int q = 0; q < kP; ++q) { a[0][q] = add2(a[0][q], d[q]); a[1][q] = fma2(d[q], f[q], a[1][q]); }
       });
     }
-    channel_sums<kV>(p, a, v0, stage, own, 2);
-    channel_sums<kV>(p, b, v0, stage, own + 1, 2);
+    channel_sums<2, kV>(p, a, v0, stage, own, s.slice);
   }
   if (s.split > 1) cluster.sync();
+  float* sum = stage;                                      // [2][slice] over the sample's, times gamma
   for (int c = threadIdx.x; c < s.slice; c += kThreads) {
     float ta = 0.0f, tb = 0.0f;
     if (s.split > 1) {
       for (int r = 0; r < s.split; ++r) {
-        const float2 o = reinterpret_cast<const float2*>(cluster.map_shared_rank(own, r))[c];
-        ta += o.x;
-        tb += o.y;
+        const float* o = cluster.map_shared_rank(own, r);
+        ta += o[c];
+        tb += o[s.slice + c];
       }
     } else {
-      ta = own[2 * c];
-      tb = own[2 * c + 1];
+      ta = own[c];
+      tb = own[s.slice + c];
     }
     if (unit.rank == 0) {
       sums[2 * unit.sample * s.channels + unit.c0 + c] = ta;
       sums[(2 * unit.sample + 1) * s.channels + unit.c0 + c] = tb;
     }
-    all[2 * c] = ta * gamma[unit.c0 + c];
-    all[2 * c + 1] = tb * gamma[unit.c0 + c];
+    const float w = coef[2 * s.slice + c];
+    sum[c] = ta * w;
+    sum[s.slice + c] = tb * w;
   }
+  if (s.split > 1) cluster.barrier_arrive();      // done with the others' sums
   __syncthreads();
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const float inv = 1.0f / ((float)s.rows * (float)s.per);
   for (int g = warp; g < groups; g += kThreads / 32) {
     float ta = 0.0f, tb = 0.0f;
     for (int c = lane; c < s.per; c += 32) {
-      ta += all[2 * (g * s.per + c)];
-      tb += all[2 * (g * s.per + c) + 1];
+      ta += sum[g * s.per + c];
+      tb += sum[s.slice + g * s.per + c];
     }
     ta = warp_sum(ta);
     tb = warp_sum(tb);
     if (lane == 0) { avg[2 * g] = ta * inv; avg[2 * g + 1] = tb * inv; }
   }
   __syncthreads();
+  // dx = d gamma r - avg(gamma d) r - n avg(gamma d n) r
+  float* last = stage;                                     // [3][slice]
+  for (int c = threadIdx.x; c < s.slice; c += kThreads) {
+    const int g = c / s.per;
+    const float r = coef[c];
+    last[c] = coef[2 * s.slice + c] * r;
+    last[s.slice + c] = -avg[2 * g] * r;
+    last[2 * s.slice + c] = -avg[2 * g + 1] * r;
+  }
+  __syncthreads();
   for (int v = p.vec; p.on(v); v += p.wide) {
     if (p.vectors > p.wide) coefficients(v);
-    // dx = d k r - avg(k d) r - n avg(k d n) r
     f2 kr[kP], a1[kP], a2[kP];
-#pragma unroll
-    for (int q = 0; q < kP; ++q) {
-      const int g = (v * kV + 2 * q) / s.per, g2 = (v * kV + (2 * q + 1) % kV) / s.per;
-      kr[q] = mul2(k[q], r_[q]);
-      a1[q] = mul2(pair(-avg[2 * g], -avg[2 * g2]), r_[q]);
-      a2[q] = mul2(pair(-avg[2 * g + 1], -avg[2 * g2 + 1]), r_[q]);
-    }
-    const int64_t at = unit.base + v * kV;
-    over_rows<2>(p.lane, p.lanes, rows, [&](int r, int u) {
-      if constexpr (kRead) rr[u] = load<T, kV>(residual + at + r * in.pitch);
-      rx[u] = in.row(r, v);
-      rd[u] = up.row(r, v);
-    }, [&](int r, int u) {
+    channels_of<kV>(last + v * kV, kr);
+    channels_of<kV>(last + s.slice + v * kV, a1);
+    channels_of<kV>(last + 2 * s.slice + v * kV, a2);
+    in.template each<2, kRead>(p, v, residual + unit.base, [&](const Pack<T, kV>(&raw)[2], const Pack<T, kV>& more, int64_t o) {
       f2 f[kP], d[kP];
-      derive(rx[u], rd[u], rr[u], f, d);
+      derive(raw, more, f, d);
 #pragma unroll
       for (int q = 0; q < kP; ++q) f[q] = fma2(f[q], a2[q], fma2(d[q], kr[q], a1[q]));
-      if (dx != nullptr) store2<T, kV>(dx + at + r * in.pitch, f);
-      if (dres != nullptr) store2<T, kV>(dres + at + r * in.pitch, d);
+      if (dx != nullptr) store2<T, kV>(dx + unit.base + o, f);
+      if (dres != nullptr) store2<T, kV>(dres + unit.base + o, d);
     });
   }
-  if (s.split > 1) cluster.sync();
+  if (s.split > 1) cluster.barrier_wait();        // nobody leaves while its sums are being read
 }
 
 // A slice has whole groups and whole vectors, and 128 bytes or more of a row where it can, so that a warp reads whole lines (more where
@@ -466,21 +494,27 @@ int launch_split(void (*kernel)(K...), int split, int64_t units, size_t smem, Sm
     default: return launch_cluster<8>(kernel, units, smem, stream, args...);
   }
 }
-constexpr int kForwardHeld = 56 * 1024, kBackwardHeld = 100 * 1024;
+// Shared memory of a CTA; the widest slices leave less of it to the rows.
+size_t fit(Shape* s, size_t row, size_t fixed) {
+  constexpr size_t kMost = 224 * 1024;
+  if (s->held * row + fixed > kMost) s->held = (int)((kMost - fixed) / row);
+  return s->held * row + fixed;
+}
+constexpr int kForwardHeld = 45 * 1024, kBackwardHeld = 64 * 1024;
 
 template <class T, int kV, int kAct, bool kAdd>
 int forward(const void* x, const void* residual, void* z, const float* gamma, const float* beta, float* stats, int64_t samples,
-            const Shape& s, void* stream) {
+            Shape s, void* stream) {
   static SmemAllowed allowed{0};
-  const size_t smem = (size_t)s.held * s.slice * sizeof(T) + sizeof(float) * (kThreads * kV + 2 * s.slice + 4 * (s.slice / s.per));
+  const size_t smem = fit(&s, (size_t)s.slice * sizeof(T), sizeof(float) * (kThreads * kV + 3 * s.slice + 4 * (s.slice / s.per)));
   return launch_split(group_norm_fwd_kernel<T, kV, kAct, kAdd>, s.split, samples * (s.channels / s.slice), smem, allowed, stream, (const T*)x,
                       (const T*)residual, (T*)z, gamma, beta, stats, s);
 }
 template <class T, int kV, int kAct, bool kAdd>
 int backward(const void* x, const void* residual, const void* dz, void* dx, void* dres, const float* gamma, const float* beta,
-             const float* stats, float* sums, int64_t samples, const Shape& s, void* stream) {
+             const float* stats, float* sums, int64_t samples, Shape s, void* stream) {
   static SmemAllowed allowed{0};
-  const size_t smem = (size_t)s.held * s.slice * sizeof(T) * 2 + sizeof(float) * (kThreads * kV + 4 * s.slice + 2 * (s.slice / s.per));
+  const size_t smem = fit(&s, (size_t)s.slice * sizeof(T) * 2, sizeof(float) * (stage_floats(kV, s.slice) + 6 * s.slice + 2 * (s.slice / s.per)));
   return launch_split(group_norm_bwd_kernel<T, kV, kAct, kAdd>, s.split, samples * (s.channels / s.slice), smem, allowed, stream, (const T*)x,
                       (const T*)residual, (const T*)dz, (T*)dx, (T*)dres, gamma, beta, stats, sums, s);
 }
