@@ -4,10 +4,13 @@
 //   loss_row = (1 - w) T^2 sum_k p_k (log p_k - log q_{i_k})  -  w log r_label
 //   dz_j     = ((1 - w) T (q_j - sum_{k: i_k = j} p_k) + w (r_j - [j = label])) / rows
 //
-// Bound by memory: a row is read from memory once (running maximum and sums), is found in L2 the second time, and its gradient is
-// written once.  The few classes that the teacher or the label names are written again, from their own sums, after the others: a
+// Bound by memory and, nearly as much, by the exponentials: a row is read from memory once (running maxima and sums), is found in L2
+// the second time, and its gradient is written once.  (Rows held in registers in between, 64 KB a block: a third of the warps, and
+// slower by a tenth.)  A block has a row, or a cluster of blocks has one where rows are fewer than SMs; their maxima and sums meet in
+// distributed shared memory.  The few classes that the teacher or the label names are written again, from their own sums, after the others: a
 // class that is named twice counts twice.  An index outside the classes is no class; a row without a teacher (or label) has no
 // such term, whatever its logits are.
+#include <cooperative_groups.h>
 #include <float.h>
 #include "launch.cuh"
 #include "rows.cuh"
@@ -16,66 +19,111 @@ namespace {
 
 using namespace esgd;
 
+namespace cg = cooperative_groups;
+
 constexpr int kMaxTop = 1024;
+constexpr int kMaxThreads = 512;
+constexpr int kThreadVectors = 8, kSplitVectors = 512;
 
 struct Args {
   const int64_t* classes_of;   // [rows][top]
   const int64_t* labels;       // [rows], or null
   const void* values;          // [rows][top]
   int values_bf16, top, classes, ld;
+  int split;                   // blocks of a row
   float inv_t, t, soft, hard;  // soft = (1 - w), hard = w
   float inv_rows;
   float* row_loss;             // [rows]
 };
 
-struct MaxOp { __device__ float operator()(float a, float b) const { return fmaxf(a, b); } };
-struct SumOp { __device__ float operator()(float a, float b) const { return a + b; } };
-template <class Op> __device__ __forceinline__ float warp_all(float v, Op op) {
+__device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-// Over the block, in a fixed order; sh: one float a warp, and its own for each call in a row.
-template <class Op> __device__ __forceinline__ float block_all(float v, Op op, float* sh) {
-  const int warps = blockDim.x / 32;
-  v = warp_all(v, op);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x / 32] = v;
-  __syncthreads();
-  float r = sh[0];
-  for (int w = 1; w < warps; ++w) r = op(r, sh[w]);
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Two vectors' maximum; a bf16 pair at a time.
+template <class T, int kV> __device__ __forceinline__ Pack<T, kV> larger(const Pack<T, kV>& a, const Pack<T, kV>& b) {
+  Pack<T, kV> r;
+  const uint32_t x[4] = {a.v.x, a.v.y, a.v.z, a.v.w}, y[4] = {b.v.x, b.v.y, b.v.z, b.v.w};
+  uint32_t z[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (sizeof(T) == 4) {
+      z[q] = __float_as_uint(fmaxf(__uint_as_float(x[q]), __uint_as_float(y[q])));
+    } else {
+      const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x[q]), *reinterpret_cast<const __nv_bfloat162*>(&y[q]));
+      z[q] = *reinterpret_cast<const uint32_t*>(&m);
+    }
+  }
+  r.v = make_uint4(z[0], z[1], z[2], z[3]);
   return r;
 }
 
-// Maximum so far and the sums of e^(z - max) (kHard) and e^((z - max) / T) about it.
-template <bool kHard> struct Running {
-  float peak = -FLT_MAX, soft = 0.0f, hard = 0.0f;
-  __device__ __forceinline__ void raise(float to, float cs, float ch) {
-    if (to > peak) {
-      soft *= exp2_approx((peak - to) * cs);
-      if constexpr (kHard) hard *= exp2_approx((peak - to) * ch);
-      peak = to;
+// The blocks' maxima (or sums) of kMany values; every thread gets them.  sh: [kMany][16], and own[kMany] for the cluster.
+template <int kMany, bool kMax> __device__ __forceinline__ void meet(float (&v)[kMany], float* sh, float* own, int split, cg::cluster_group& cluster) {
+  const int warps = blockDim.x / 32;
+#pragma unroll
+  for (int i = 0; i < kMany; ++i) {
+    v[i] = kMax ? warp_max(v[i]) : warp_sum(v[i]);
+    if ((threadIdx.x & 31) == 0) sh[i * 16 + threadIdx.x / 32] = v[i];
+  }
+  __syncthreads();
+  const int w = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < kMany; ++i) {
+    float r = w < warps ? sh[i * 16 + w] : kMax ? -INFINITY : 0.0f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, r, o);
+      r = kMax ? fmaxf(r, other) : r + other;
+    }
+    v[i] = r;
+    if (split > 1 && threadIdx.x == 0) own[i] = r;
+  }
+  if (split > 1) {
+    cluster.sync();
+#pragma unroll
+    for (int i = 0; i < kMany; ++i) {
+      float r = cluster.map_shared_rank(own, 0)[i];
+      for (int k = 1; k < split; ++k) {
+        const float o = cluster.map_shared_rank(own, k)[i];
+        r = kMax ? fmaxf(r, o) : r + o;
+      }
+      v[i] = r;
     }
   }
-  __device__ __forceinline__ void add(float x, float cs, float ch) {
-    soft += exp2_approx((x - peak) * cs);
-    if constexpr (kHard) hard += exp2_approx((x - peak) * ch);
-  }
-};
+}
 
 template <class T, bool kHard, bool kGrad>
-__global__ void __launch_bounds__(512) distill_kernel(const T* __restrict__ logits, T* __restrict__ grad, Args a) {
+__global__ void __launch_bounds__(kMaxThreads, 4) distill_kernel(const T* __restrict__ logits, T* __restrict__ grad, Args a) {
   pdl_enter();
-  constexpr int kV = vector_of<T>();
-  extern __shared__ float smem[];
-  float* prob = smem;                                       // [top]
-  int* index = reinterpret_cast<int*>(smem + a.top);        // [top], -1: none
-  __shared__ float sh[6][16];
-  const int row = blockIdx.x, tid = threadIdx.x, threads = blockDim.x;
+  constexpr int kV = vector_of<T>(), kP = kV / 2;
+  extern __shared__ int4 smem4[];
+  const int fours = (a.top + 3) / 4;
+  int* index = reinterpret_cast<int*>(smem4);               // [top], -1: none; -2 up to a multiple of four
+  float* prob = reinterpret_cast<float*>(smem4 + fours);    // [top]
+  __shared__ float sh[3][3 * 16], own[3][3];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = a.split > 1 ? (int)cluster.block_rank() : 0;
+  const int row = blockIdx.x / a.split, tid = threadIdx.x, threads = blockDim.x;
   const T* x = logits + (int64_t)row * a.ld;
   const float cs = a.inv_t * kLog2e, ch = kLog2e;
 
-  // the teacher's distribution
-  float top_peak = -INFINITY;
+  // vectors from the first 16-byte boundary on, this block's share of them, and the single elements at the ends (the first block's)
+  const int head = min(a.classes, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+  const int vectors = (a.classes - head) / kV, tail = head + vectors * kV, ends = rank == 0 ? head + a.classes - tail : 0;
+  const int from = (int)((int64_t)vectors * rank / a.split), to = (int)((int64_t)vectors * (rank + 1) / a.split);
+  const T* base = x + head;
+
+  // the teacher's logits
+  float peaks[2] = {-FLT_MAX, -INFINITY};
+  if (tid < 4 * fours - a.top) index[a.top + tid] = -2;
   for (int k = tid; k < a.top; k += threads) {
     const int64_t at = (int64_t)row * a.top + k, c = a.classes_of[at];
     const float v = a.values_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.values)[at])
@@ -83,82 +131,123 @@ __global__ void __launch_bounds__(512) distill_kernel(const T* __restrict__ logi
     const bool is = c >= 0 && c < a.classes && v != -INFINITY;
     prob[k] = v;
     index[k] = is ? (int)c : -1;
-    if (is) top_peak = fmaxf(top_peak, v);
+    if (is) peaks[1] = fmaxf(peaks[1], v);
   }
-  top_peak = block_all(top_peak, MaxOp(), sh[0]);
-  float top_sum = 0.0f;
-  for (int k = tid; k < a.top; k += threads)
-    if (index[k] >= 0) top_sum += exp_fine((prob[k] - top_peak) * a.inv_t);
-  top_sum = block_all(top_sum, SumOp(), sh[1]);
-  const bool taught = a.soft != 0.0f && top_peak != -INFINITY;
   int64_t label = -1;
   if constexpr (kHard) {
     label = a.labels[row];
     if (label < 0 || label >= a.classes) label = -1;
   }
-
-  // the row's maximum and sums; vectors from the first 16-byte boundary on
-  const int head = min(a.classes, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
-  const int vectors = (a.classes - head) / kV, tail = head + vectors * kV;
-  Running<kHard> run;
-  if (taught || label >= 0) {
-    for (int i = tid; i < vectors; i += 2 * threads) {
-      const bool two = i + threads < vectors;
-      const Pack<T, kV> r0 = load<T, kV>(x + head + i * kV);
-      Pack<T, kV> r1 = r0;
-      if (two) r1 = load<T, kV>(x + head + (i + threads) * kV);
-      float f[kV], g[kV];
-      unpack<T, kV>(r0, f);
-      unpack<T, kV>(r1, g);
-      float m = f[0];
-#pragma unroll
-      for (int q = 0; q < kV; ++q) m = fmaxf(m, fmaxf(f[q], g[q]));
-      run.raise(m, cs, ch);
-#pragma unroll
-      for (int q = 0; q < kV; ++q) run.add(f[q], cs, ch);
-      if (two) {
-#pragma unroll
-        for (int q = 0; q < kV; ++q) run.add(g[q], cs, ch);
-      }
+  // a thread's maximum so far, and its sums of e^((z - max) / T) and e^(z - max) about it
+  const f2 cs2 = pair(cs, cs), ch2 = pair(ch, ch);
+  f2 soft = 0, hard = 0;
+  auto raise = [&](float m) {
+    if (m > peaks[0]) {
+      soft = mul2(soft, exp2_approx((peaks[0] - m) * cs));
+      if constexpr (kHard) hard = mul2(hard, exp2_approx((peaks[0] - m) * ch));
+      peaks[0] = m;
     }
-    for (int i = tid; i < head + a.classes - tail; i += threads) {
-      const float f = as_float(x[i < head ? i : tail + i - head]);
-      run.raise(f, cs, ch);
-      run.add(f, cs, ch);
+  };
+  auto add = [&](const f2 (&f)[kP]) {
+    const f2 minus = pair(-peaks[0], -peaks[0]);
+#pragma unroll
+    for (int q = 0; q < kP; ++q) {
+      const f2 d = add2(f[q], minus);
+      soft = add2(soft, exp2_2(mul2(d, cs2)));
+      if constexpr (kHard) hard = add2(hard, exp2_2(mul2(d, ch2)));
     }
+  };
+  auto largest = [&](const Pack<T, kV>& m) {
+    f2 f[kP];
+    unpack2<T, kV>(m, f);
+    float r = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < kP; ++q) r = fmaxf(r, fmaxf(halves(f[q]).x, halves(f[q]).y));
+    return r;
+  };
+  int i = from + tid;
+  for (; i + threads < to; i += 2 * threads) {
+    const Pack<T, kV> r0 = load<T, kV>(base + (int64_t)i * kV), r1 = load<T, kV>(base + (int64_t)(i + threads) * kV);
+    raise(largest(larger<T, kV>(r0, r1)));
+    f2 f[kP];
+    unpack2<T, kV>(r0, f);
+    add(f);
+    unpack2<T, kV>(r1, f);
+    add(f);
   }
-  const float peak = block_all(run.peak, MaxOp(), sh[2]);
-  run.raise(peak, cs, ch);
-  const float soft_sum = block_all(run.soft, SumOp(), sh[3]);
-  float hard_sum = 1.0f;
-  if constexpr (kHard) hard_sum = block_all(run.hard, SumOp(), sh[4]);
-  const float log_soft = __logf(soft_sum);
+  if (i < to) {
+    const Pack<T, kV> r = load<T, kV>(base + (int64_t)i * kV);
+    raise(largest(r));
+    f2 f[kP];
+    unpack2<T, kV>(r, f);
+    add(f);
+  }
+  float sums[3] = {halves(soft).x + halves(soft).y, halves(hard).x + halves(hard).y, 0.0f};
+  float own_end = peaks[0];
+  for (int e = tid; e < ends; e += threads) {
+    const float z = as_float(x[e < head ? e : tail + e - head]);
+    if (z > own_end) {
+      sums[0] *= exp2_approx((own_end - z) * cs);
+      sums[1] *= exp2_approx((own_end - z) * ch);
+      own_end = z;
+    }
+    sums[0] += exp2_approx((z - own_end) * cs);
+    if constexpr (kHard) sums[1] += exp2_approx((z - own_end) * ch);
+  }
+  peaks[0] = own_end;
+  meet<2, true>(peaks, sh[0], own[0], a.split, cluster);
+  const float peak = peaks[0], top_peak = peaks[1];
+  const bool taught = a.soft != 0.0f && top_peak != -INFINITY, any = taught || label >= 0;
+  const f2 minus = pair(-peak, -peak);
+  sums[0] *= exp2_approx((own_end - peak) * cs);
+  if constexpr (kHard) sums[1] *= exp2_approx((own_end - peak) * ch);
+  if (rank == 0)
+    for (int k = tid; k < a.top; k += threads)
+      if (index[k] >= 0) sums[2] += exp_fine((prob[k] - top_peak) * a.inv_t);
+  meet<3, false>(sums, sh[1], own[1], a.split, cluster);
+  const float log_soft = __logf(sums[0]);
 
   // loss: log p_k - log q_k = (v_k - v_max) / T - log(sum) - (z_k - z_max) / T + log(sum_z)
   float kl = 0.0f;
-  const float log_top = taught ? __logf(top_sum) : 0.0f, inv_top = taught ? 1.0f / top_sum : 0.0f;
+  const float log_top = taught ? __logf(sums[2]) : 0.0f, inv_top = taught ? 1.0f / sums[2] : 0.0f;
   for (int k = tid; k < a.top; k += threads) {
     float p = 0.0f;
     if (taught && index[k] >= 0) {
       const float v = (prob[k] - top_peak) * a.inv_t;
       p = exp_fine(v) * inv_top;
-      if (p != 0.0f) kl += p * ((v - log_top) - ((as_float(x[index[k]]) - peak) * a.inv_t - log_soft));
+      if (rank == 0 && p != 0.0f) kl += p * ((v - log_top) - ((as_float(x[index[k]]) - peak) * a.inv_t - log_soft));
     }
     prob[k] = p;
   }
-  kl = block_all(kl, SumOp(), sh[5]);        // prob[] is whole behind its barrier
-  if (tid == 0) {
-    float loss = taught ? a.soft * a.t * a.t * kl : 0.0f;
-    if constexpr (kHard)
-      if (label >= 0) loss += a.hard * (__logf(hard_sum) - (as_float(x[label]) - peak));
-    a.row_loss[row] = loss;
-  }
+  kl = warp_sum(kl);
+  if ((tid & 31) == 0) sh[2][tid / 32] = kl;
+  if (a.split > 1) cluster.barrier_arrive();                // done with the others' sums
+
+  const float ks = taught ? a.soft * a.t * a.inv_rows : 0.0f, kh = kHard && label >= 0 ? a.hard * a.inv_rows : 0.0f;
   if constexpr (kGrad) {
     T* d = grad + (int64_t)row * a.ld;
-    const float ks = taught ? a.soft * a.t * a.inv_rows : 0.0f, kh = kHard && label >= 0 ? a.hard * a.inv_rows : 0.0f;
-    const float fs = ks != 0.0f ? ks / soft_sum : 0.0f, fh = kh != 0.0f ? kh / hard_sum : 0.0f;
-    const bool any = ks != 0.0f || kh != 0.0f;
-    auto dense = [&](float z) {
+    const float fs = ks != 0.0f ? ks / sums[0] : 0.0f, fh = kh != 0.0f ? kh / sums[1] : 0.0f;
+    const f2 fs2 = pair(fs, fs), fh2 = pair(fh, fh);
+    auto dense = [&](const Pack<T, kV>& r, T* at) {
+      f2 f[kP];
+      unpack2<T, kV>(r, f);
+#pragma unroll
+      for (int q = 0; q < kP; ++q) {
+        const f2 e = add2(f[q], minus);
+        f[q] = mul2(exp2_2(mul2(e, cs2)), fs2);
+        if constexpr (kHard) f[q] = fma2(exp2_2(mul2(e, ch2)), fh2, f[q]);
+        if (!any) f[q] = 0;
+      }
+      store2<T, kV>(at, f);
+    };
+    int i = from + tid;
+    for (; i + threads < to; i += 2 * threads) {
+      const Pack<T, kV> r0 = load<T, kV>(base + (int64_t)i * kV), r1 = load<T, kV>(base + (int64_t)(i + threads) * kV);
+      dense(r0, d + head + (int64_t)i * kV);
+      dense(r1, d + head + (int64_t)(i + threads) * kV);
+    }
+    if (i < to) dense(load<T, kV>(base + (int64_t)i * kV), d + head + (int64_t)i * kV);
+    auto one = [&](float z) {
       float v = 0.0f;
       if (any) {
         v = exp2_approx((z - peak) * cs) * fs;
@@ -166,39 +255,50 @@ __global__ void __launch_bounds__(512) distill_kernel(const T* __restrict__ logi
       }
       return v;
     };
-    for (int i = tid; i < vectors; i += threads) {
-      float f[kV];
-      unpack<T, kV>(load<T, kV>(x + head + i * kV), f);
-#pragma unroll
-      for (int q = 0; q < kV; ++q) f[q] = dense(f[q]);
-      store<T, kV>(d + head + i * kV, f);
-    }
-    for (int i = tid; i < head + a.classes - tail; i += threads) {
+    for (int i = tid; i < ends; i += threads) {
       const int c = i < head ? i : tail + i - head;
-      d[c] = as_type<T>(dense(as_float(x[c])));
+      d[c] = as_type<T>(one(as_float(x[c])));
     }
     __syncthreads();
+    // the named classes among this block's
+    auto mine = [&](int c) { return c < head || c >= tail ? rank == 0 : (c - head) / kV >= from && (c - head) / kV < to; };
     if (taught) {
       for (int k = tid; k < a.top; k += threads) {
         const int c = index[k];
-        if (c < 0) continue;
-        float p = 0.0f;
+        if (c < 0 || !mine(c)) continue;
+        float p = prob[k];
         bool first = true;
-        for (int j = 0; j < a.top; ++j)
-          if (index[j] == c) {
-            if (j < k) { first = false; break; }
-            p += prob[j];
+        for (int j = 0; j < fours; ++j) {
+          const int4 o = smem4[j];
+          if (o.x != c && o.y != c && o.z != c && o.w != c) continue;
+          const int same[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (same[i] != c || 4 * j + i == k) continue;
+            if (4 * j + i < k) first = false;
+            else p += prob[4 * j + i];
           }
-        if (first) d[c] = as_type<T>(dense(as_float(x[c])) - ks * p - (c == label ? kh : 0.0f));
+        }
+        if (first) d[c] = as_type<T>(one(as_float(x[c])) - ks * p - (c == label ? kh : 0.0f));
       }
     }
     if (kHard && label >= 0) {       // a label that the teacher does not name
       bool named = false;
       if (taught)
         for (int k = tid; k < a.top; k += threads) named = named || index[k] == (int)label;
-      if (!__syncthreads_or(named) && tid == 0) d[label] = as_type<T>(dense(as_float(x[label])) - kh);
+      if (!__syncthreads_or(named) && tid == 0 && mine((int)label)) d[label] = as_type<T>(one(as_float(x[label])) - kh);
     }
+  } else {
+    __syncthreads();
   }
+  if (tid == 0 && rank == 0) {
+    for (int w = 1; w < threads / 32; ++w) kl += sh[2][w];
+    float loss = taught ? a.soft * a.t * a.t * kl : 0.0f;
+    if constexpr (kHard)
+      if (label >= 0) loss += a.hard * (__logf(sums[1]) - (as_float(x[label]) - peak));
+    a.row_loss[row] = loss;
+  }
+  if (a.split > 1) cluster.barrier_wait();                  // nobody leaves while its sums are being read
 }
 
 // The rows' mean in a fixed order.
@@ -238,18 +338,30 @@ __global__ void __launch_bounds__(256) distill_scale_kernel(const T* in, T* out,
   }
 }
 
+// Eight vectors a thread or more; rows that are fewer than SMs are spread over more blocks as long as these have something to do.
+template <class T, class... K> int launch_row(void (*kernel)(K...), const T* x, T* d, Args a, int rows, void* stream) {
+  const int vectors = (a.classes + vector_of<T>() - 1) / vector_of<T>();
+  a.split = 1;
+  while (a.split < 8 && rows * a.split < 2 * sm_count() && vectors > a.split * kSplitVectors) a.split *= 2;
+  int threads = 128;
+  while (threads < kMaxThreads && vectors > a.split * threads * kThreadVectors) threads *= 2;
+  const dim3 grid((unsigned)(rows * a.split));
+  const size_t smem = (size_t)((a.top + 3) / 4 * 4) * 8;
+  switch (a.split) {
+    case 1: return launch<1>(kernel, grid, threads, smem, stream, x, d, a);
+    case 2: return launch<2>(kernel, grid, threads, smem, stream, x, d, a);
+    case 4: return launch<4>(kernel, grid, threads, smem, stream, x, d, a);
+    default: return launch<8>(kernel, grid, threads, smem, stream, x, d, a);
+  }
+}
 template <class T>
 int launch_rows(const void* logits, void* grad, const Args& a, int rows, void* stream) {
-  const int threads = a.classes <= 1024 * vector_of<T>() / 4 ? 128 : 512;
-  const size_t smem = (size_t)a.top * 8;
   const bool hard = a.labels != nullptr && a.hard != 0.0f;
   const T* x = (const T*)logits;
   T* d = (T*)grad;
   if (grad != nullptr)
-    return hard ? launch(distill_kernel<T, true, true>, dim3(rows), threads, smem, stream, x, d, a)
-                : launch(distill_kernel<T, false, true>, dim3(rows), threads, smem, stream, x, d, a);
-  return hard ? launch(distill_kernel<T, true, false>, dim3(rows), threads, smem, stream, x, d, a)
-              : launch(distill_kernel<T, false, false>, dim3(rows), threads, smem, stream, x, d, a);
+    return hard ? launch_row(distill_kernel<T, true, true>, x, d, a, rows, stream) : launch_row(distill_kernel<T, false, true>, x, d, a, rows, stream);
+  return hard ? launch_row(distill_kernel<T, true, false>, x, d, a, rows, stream) : launch_row(distill_kernel<T, false, false>, x, d, a, rows, stream);
 }
 
 }  // namespace
@@ -262,8 +374,8 @@ int esgd_distill_max_top() { return kMaxTop; }
 int esgd_distill(const void* logits, void* grad, int is_bf16, const void* values, int values_bf16, const int64_t* classes_of,
                  const int64_t* labels, int rows, int classes, int ld, int top, float temperature, float hard_weight, float* row_loss,
                  float* loss, void* stream) {
-  if (rows <= 0 || classes <= 0 || top < 0 || top > kMaxTop) return (int)cudaErrorInvalidValue;
-  const Args a = {classes_of, labels, values, values_bf16, top, classes, ld, 1.0f / temperature, temperature, 1.0f - hard_weight,
+  if (rows <= 0 || classes <= 0 || top < 0 || top > kMaxTop || rows > (1 << 27)) return (int)cudaErrorInvalidValue;
+  const Args a = {classes_of, labels, values, values_bf16, top, classes, ld, 1, 1.0f / temperature, temperature, 1.0f - hard_weight,
                   hard_weight, 1.0f / (float)rows, row_loss};
   int rc = is_bf16 ? launch_rows<__nv_bfloat16>(logits, grad, a, rows, stream) : launch_rows<float>(logits, grad, a, rows, stream);
   if (rc == 0) rc = launch(distill_mean_kernel, dim3(1), 1024, 0, stream, row_loss, rows, loss);
