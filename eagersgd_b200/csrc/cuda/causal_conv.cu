@@ -3,8 +3,9 @@
 //   pre[t] = bias + sum_k w[k] x[t - K + 1 + k],   y[t] = act(pre[t])
 //   dpre = dy act'(pre);  dx[t] = sum_j w[K - 1 - j] dpre[t + j];  dw[k] = sum dpre[t] x[t - K + 1 + k];  dbias = sum dpre
 //
-// Bound by memory.  A thread has a vector of channels and a run of steps, the window in registers: of every run only the K - 1
-// inputs ahead of it are read twice (the backward pass makes the K - 1 dpre behind it again).
+// Bound by memory.  A thread has four channels and a run of steps, the window in registers: of every run only the K - 1 inputs ahead
+// of it are read twice (the backward pass makes the K - 1 dpre behind it again).  Eight channels a thread took twice the registers,
+// and half the warps were not enough loads in flight.
 #include "launch.cuh"
 #include "rows.cuh"
 
@@ -13,6 +14,7 @@ namespace {
 using namespace esgd;
 
 constexpr int kThreads = 256;
+constexpr int kAhead = 4;            // steps that are loaded at a time
 
 struct Conv {
   int64_t batch, length;
@@ -53,179 +55,198 @@ template <int kV> struct Spot {
   }
 };
 
-template <class T, int kV> __device__ __forceinline__ void input(const T* x, const T* state, const Conv& p, int64_t b, int64_t t, int c,
-                                                                 int taps, float (&f)[kV]) {
+template <class T, int kV>
+__device__ __forceinline__ void input(const T* x, const T* state, const Conv& p, int64_t b, int64_t t, int c, int taps, f2 (&f)[PairsOf<kV>::n]) {
   if (t >= 0) {
-    unpack<T, kV>(load<T, kV>(x + b * p.xb + t * p.xt + c), f);
+    unpack2<T, kV>(load<T, kV>(x + b * p.xb + t * p.xt + c), f);
   } else if (state != nullptr) {
-    unpack<T, kV>(load<T, kV>(state + (b * (taps - 1) + t + taps - 1) * p.channels + c), f);
+    unpack2<T, kV>(load<T, kV>(state + (b * (taps - 1) + t + taps - 1) * p.channels + c), f);
   } else {
 #pragma unroll
-    for (int q = 0; q < kV; ++q) f[q] = 0.0f;
+    for (int q = 0; q < PairsOf<kV>::n; ++q) f[q] = 0;
   }
 }
+template <int kV, int kTaps> struct Filter {
+  static constexpr int kP = PairsOf<kV>::n;
+  f2 w[kTaps][kP], bias[kP];
+  // c: the first of the channels, whose taps lie in a row.
+  __device__ Filter(const float* weight, const float* bias_of, int c) {
+    float taps[kV * kTaps], b[kV];
+    const float* from = weight + (int64_t)c * kTaps;
+    if (kV == 4 && ((uintptr_t)from & 15) == 0) {
+#pragma unroll
+      for (int k = 0; k < kTaps * kV / 4; ++k) {
+        const float4 v = reinterpret_cast<const float4*>(from)[k];
+        taps[4 * k % (kV * kTaps)] = v.x;
+        taps[(4 * k + 1) % (kV * kTaps)] = v.y;
+        taps[(4 * k + 2) % (kV * kTaps)] = v.z;
+        taps[(4 * k + 3) % (kV * kTaps)] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kV * kTaps; ++i) taps[i] = from[i];
+    }
+#pragma unroll
+    for (int q = 0; q < kV; ++q) b[q] = bias_of != nullptr ? bias_of[c + q] : 0.0f;
+#pragma unroll
+    for (int q = 0; q < kP; ++q) {
+      bias[q] = pair(b[2 * q], kV > 1 ? b[(2 * q + 1) % kV] : 0.0f);
+#pragma unroll
+      for (int k = 0; k < kTaps; ++k) w[k][q] = pair(taps[2 * q * kTaps + k], kV > 1 ? taps[((2 * q + 1) * kTaps + k) % (kV * kTaps)] : 0.0f);
+    }
+  }
+  __device__ __forceinline__ f2 at(const f2 (&win)[kTaps][kP], int q) const {
+    f2 pre = bias[q];
+#pragma unroll
+    for (int k = 0; k < kTaps; ++k) pre = fma2(w[k][q], win[k][q], pre);
+    return pre;
+  }
+};
 
 template <class T, int kV, int kTaps, int kAct>
 __global__ void __launch_bounds__(kThreads) causal_conv_fwd_kernel(const T* __restrict__ x, const T* __restrict__ state, T* __restrict__ y,
                                                                    T* __restrict__ state_out, Conv p) {
   pdl_enter();
+  constexpr int kP = PairsOf<kV>::n;
   const Spot<kV> s(p);
   if (!s.on) return;
   if (state_out != nullptr && s.first == (int64_t)s.run * p.steps)        // blocks of the first steps
     for (int i = s.run; i < kTaps - 1; i += p.runs) {
-      float f[kV];
+      f2 f[kP];
       input<T, kV>(x, state, p, s.b, s.len - (kTaps - 1) + i, s.c, kTaps, f);
-      store<T, kV>(state_out + (s.b * (kTaps - 1) + i) * p.channels + s.c, f);
+      store2<T, kV>(state_out + (s.b * (kTaps - 1) + i) * p.channels + s.c, f);
     }
   if (s.first >= p.length) return;
-  float w[kTaps][kV], bias[kV], win[kTaps][kV];
+  const int steps = (int)(s.last - s.first), live = (int)(s.len - s.first < 0 ? 0 : s.len - s.first < steps ? s.len - s.first : steps);
+  const T* in = x + s.b * p.xb + s.first * p.xt + s.c;
+  T* out = y + (s.b * p.length + s.first) * p.channels + s.c;
+  if (live > 0) {
+    const Filter<kV, kTaps> filter(p.weight, p.bias, s.c);
+    f2 win[kTaps][kP];
 #pragma unroll
-  for (int q = 0; q < kV; ++q) {
-    bias[q] = p.bias != nullptr ? p.bias[s.c + q] : 0.0f;
+    for (int k = 0; k < kTaps - 1; ++k) input<T, kV>(x, state, p, s.b, s.first - (kTaps - 1) + k, s.c, kTaps, win[k + 1]);
+    for (int t = 0; t < live; t += kAhead) {
+      Pack<T, kV> raw[kAhead];
 #pragma unroll
-    for (int k = 0; k < kTaps; ++k) w[k][q] = p.weight[(s.c + q) * kTaps + k];
-  }
+      for (int u = 0; u < kAhead; ++u)
+        if (t + u < live) raw[u] = load<T, kV>(in + u * p.xt);
+      in += kAhead * p.xt;
 #pragma unroll
-  for (int k = 0; k < kTaps - 1; ++k) {
-    if (s.first < s.len) {
-      input<T, kV>(x, state, p, s.b, s.first - (kTaps - 1) + k, s.c, kTaps, win[k + 1]);
-    } else {
+      for (int u = 0; u < kAhead; ++u) {
+        if (t + u >= live) break;
+        f2 f[kP];
 #pragma unroll
-      for (int q = 0; q < kV; ++q) win[k + 1][q] = 0.0f;
-    }
-  }
-  const T* in = x + s.b * p.xb + s.c;
-  T* out = y + s.b * p.length * p.channels + s.c;
-  for (int64_t t = s.first; t < s.last; t += 4) {
-    Pack<T, kV> raw[4];
+        for (int q = 0; q < kP; ++q)
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (t + u < s.last && t + u < s.len) raw[u] = load<T, kV>(in + (t + u) * p.xt);
+          for (int k = 0; k < kTaps - 1; ++k) win[k][q] = win[k + 1][q];
+        unpack2<T, kV>(raw[u], win[kTaps - 1]);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (t + u >= s.last) break;
-      float f[kV];
-#pragma unroll
-      for (int q = 0; q < kV; ++q) f[q] = 0.0f;
-      if (t + u < s.len) {
-#pragma unroll
-        for (int k = 0; k < kTaps - 1; ++k)
-#pragma unroll
-          for (int q = 0; q < kV; ++q) win[k][q] = win[k + 1][q];
-        unpack<T, kV>(raw[u], win[kTaps - 1]);
-#pragma unroll
-        for (int q = 0; q < kV; ++q) {
-          float pre = bias[q];
-#pragma unroll
-          for (int k = 0; k < kTaps; ++k) pre = fmaf(w[k][q], win[k][q], pre);
-          f[q] = activate<kAct>(pre);
-        }
+        for (int q = 0; q < kP; ++q) f[q] = activate2<kAct>(filter.at(win, q));
+        store2<T, kV>(out + (int64_t)u * p.channels, f);
       }
-      store<T, kV>(out + (t + u) * p.channels, f);
+      out += (int64_t)kAhead * p.channels;
     }
   }
+  const f2 zero[kP] = {};
+  for (int t = live; t < steps; ++t) store2<T, kV>(y + (s.b * p.length + s.first + t) * p.channels + s.c, zero);
 }
 
 // sums [blocks of a channel][channels * K + channels]: each block's share of dw and dbias.
 template <class T, int kV, int kTaps, int kAct>
-__global__ void __launch_bounds__(kThreads) causal_conv_bwd_kernel(const T* __restrict__ x, const T* __restrict__ state,
-                                                                   const T* __restrict__ dy, T* __restrict__ dx, float* __restrict__ sums,
-                                                                   Conv p) {
+__global__ void __launch_bounds__(kThreads, 2) causal_conv_bwd_kernel(const T* __restrict__ x, const T* __restrict__ state,
+                                                                      const T* __restrict__ dy, T* __restrict__ dx, float* __restrict__ sums,
+                                                                      Conv p) {
   pdl_enter();
-  __shared__ float stage[kThreads * kV];
+  constexpr int kP = PairsOf<kV>::n;
+  __shared__ float stage[(kTaps + 1) * kThreads * kV];
   const Spot<kV> s(p);
-  float dw[kTaps + 1][kV];
+  f2 dw[kTaps + 1][kP];
 #pragma unroll
   for (int k = 0; k <= kTaps; ++k)
 #pragma unroll
-    for (int q = 0; q < kV; ++q) dw[k][q] = 0.0f;
+    for (int q = 0; q < kP; ++q) dw[k][q] = 0;
   if (s.on && s.first < p.length) {
-    float w[kTaps][kV], bias[kV], win[kTaps][kV], dp[kTaps][kV];
+    // steps of the run, and up to K - 1 behind it for the gradients of its last inputs
+    const int steps = (int)(s.last - s.first), ahead = (int)(s.len - s.first < 0 ? 0 : s.len - s.first < steps + kTaps - 1 ? s.len - s.first : steps + kTaps - 1);
+    const T* in = x + s.b * p.xb + s.first * p.xt + s.c;
+    const int64_t row = (s.b * p.length + s.first) * p.channels + s.c;
+    const T* up = dy + row;
+    T* out = dx + row - (int64_t)(kTaps - 1) * p.channels;
+    int t = 0;
+    if (ahead > 0) {
+      const Filter<kV, kTaps> filter(p.weight, p.bias, s.c);
+      f2 win[kTaps][kP], dp[kTaps][kP];
 #pragma unroll
-    for (int q = 0; q < kV; ++q) {
-      bias[q] = p.bias != nullptr ? p.bias[s.c + q] : 0.0f;
+      for (int q = 0; q < kP; ++q)
 #pragma unroll
-      for (int k = 0; k < kTaps; ++k) w[k][q] = p.weight[(s.c + q) * kTaps + k];
-    }
-#pragma unroll
-    for (int k = 0; k < kTaps; ++k)
-#pragma unroll
-      for (int q = 0; q < kV; ++q) win[k][q] = dp[k][q] = 0.0f;
-    if (s.first < s.len)
+        for (int k = 0; k < kTaps; ++k) win[k][q] = dp[k][q] = 0;
 #pragma unroll
       for (int k = 0; k < kTaps - 1; ++k) input<T, kV>(x, state, p, s.b, s.first - (kTaps - 1) + k, s.c, kTaps, win[k + 1]);
-    const T* in = x + s.b * p.xb + s.c;
-    const T* up = dy + s.b * p.length * p.channels + s.c;
-    T* out = dx + s.b * p.length * p.channels + s.c;
-    for (int64_t t = s.first; t < s.last + kTaps - 1; t += 4) {
-      Pack<T, kV> rx[4], rd[4];
+      for (; t < steps + kTaps - 1; t += kAhead) {
+        Pack<T, kV> rx[kAhead], rd[kAhead];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (t + u < s.last + kTaps - 1 && t + u < s.len) {
-          rx[u] = load<T, kV>(in + (t + u) * p.xt);
-          rd[u] = load<T, kV>(up + (t + u) * p.channels);
-        }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t now = t + u;
-        if (now >= s.last + kTaps - 1) break;
-#pragma unroll
-        for (int k = 0; k < kTaps - 1; ++k)
-#pragma unroll
-          for (int q = 0; q < kV; ++q) { win[k][q] = win[k + 1][q]; dp[k][q] = dp[k + 1][q]; }
-        if (now < s.len) {
-          float d[kV];
-          unpack<T, kV>(rx[u], win[kTaps - 1]);
-          unpack<T, kV>(rd[u], d);
-#pragma unroll
-          for (int q = 0; q < kV; ++q) {
-            if constexpr (kAct != kActNone) {
-              float pre = bias[q];
-#pragma unroll
-              for (int k = 0; k < kTaps; ++k) pre = fmaf(w[k][q], win[k][q], pre);
-              d[q] *= slope<kAct>(pre);
-            }
-            dp[kTaps - 1][q] = d[q];
-            if (now < s.last) {
-              dw[kTaps][q] += d[q];
-#pragma unroll
-              for (int k = 0; k < kTaps; ++k) dw[k][q] = fmaf(d[q], win[k][q], dw[k][q]);
-            }
+        for (int u = 0; u < kAhead; ++u)
+          if (t + u < ahead) {
+            rx[u] = load<T, kV>(in + u * p.xt);
+            rd[u] = load<T, kV>(up + (int64_t)u * p.channels);
           }
-        } else {
+        in += kAhead * p.xt;
+        up += (int64_t)kAhead * p.channels;
 #pragma unroll
-          for (int q = 0; q < kV; ++q) dp[kTaps - 1][q] = 0.0f;
-        }
-        const int64_t back = now - (kTaps - 1);
-        if (back >= s.first && dx != nullptr) {
-          float f[kV];
+        for (int u = 0; u < kAhead; ++u) {
+          if (t + u >= steps + kTaps - 1) break;
 #pragma unroll
-          for (int q = 0; q < kV; ++q) {
-            f[q] = 0.0f;
+          for (int q = 0; q < kP; ++q)
 #pragma unroll
-            for (int j = 0; j < kTaps; ++j) f[q] = fmaf(w[kTaps - 1 - j][q], dp[j][q], f[q]);
+            for (int k = 0; k < kTaps - 1; ++k) { win[k][q] = win[k + 1][q]; dp[k][q] = dp[k + 1][q]; }
+          if (t + u < ahead) {
+            f2 d[kP];
+            unpack2<T, kV>(rx[u], win[kTaps - 1]);
+            unpack2<T, kV>(rd[u], d);
+#pragma unroll
+            for (int q = 0; q < kP; ++q) {
+              if constexpr (kAct != kActNone) d[q] = mul2(d[q], slope2<kAct>(filter.at(win, q)));
+              dp[kTaps - 1][q] = d[q];
+              if (t + u < steps) {
+                dw[kTaps][q] = add2(dw[kTaps][q], d[q]);
+#pragma unroll
+                for (int k = 0; k < kTaps; ++k) dw[k][q] = fma2(d[q], win[k][q], dw[k][q]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < kP; ++q) dp[kTaps - 1][q] = 0;
           }
-          store<T, kV>(out + back * p.channels, f);
+          if (t + u >= kTaps - 1 && dx != nullptr) {
+            f2 f[kP];
+#pragma unroll
+            for (int q = 0; q < kP; ++q) {
+              f[q] = mul2(filter.w[kTaps - 1][q], dp[0][q]);
+#pragma unroll
+              for (int j = 1; j < kTaps; ++j) f[q] = fma2(filter.w[kTaps - 1 - j][q], dp[j][q], f[q]);
+            }
+            store2<T, kV>(out + (int64_t)u * p.channels, f);
+          }
         }
+        out += (int64_t)kAhead * p.channels;
       }
+    } else if (dx != nullptr) {
+      const f2 zero[kP] = {};
+      for (; t < steps; ++t) store2<T, kV>(dx + row + (int64_t)t * p.channels, zero);
     }
   }
   if (sums == nullptr) return;
   float* part = sums + (int64_t)(blockIdx.x / p.vec_blocks) * p.channels * (kTaps + 1);
 #pragma unroll
-  for (int k = 0; k <= kTaps; ++k) {
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kV; ++q) stage[threadIdx.x * kV + q] = dw[k][q];
-    __syncthreads();
-    const int vb = (int)(blockIdx.x % p.vec_blocks);
-    for (int i = threadIdx.x; i < p.lanes * kV; i += kThreads) {
-      const int c = vb * p.lanes * kV + i;
-      if (c >= p.channels) break;
-      float t = 0.0f;
-      for (int r = 0; r < p.runs; ++r) t += stage[r * p.lanes * kV + i];
-      part[k < kTaps ? c * kTaps + k : p.channels * kTaps + c] = t;
-    }
+  for (int k = 0; k <= kTaps; ++k) store2<float, kV>(stage + (k * kThreads + threadIdx.x) * kV, dw[k]);
+  __syncthreads();
+  const int wide = p.lanes * kV, c0 = (int)(blockIdx.x % p.vec_blocks) * wide;
+  for (int i = threadIdx.x; i < (kTaps + 1) * wide; i += kThreads) {
+    const int k = i / wide, c = i - k * wide;
+    if (c0 + c >= p.channels) continue;
+    float t = 0.0f;
+    for (int r = 0; r < p.runs; ++r) t += stage[(k * kThreads + r * p.lanes) * kV + c];
+    part[k < kTaps ? (c0 + c) * kTaps + k : p.channels * kTaps + c0 + c] = t;
   }
 }
 
@@ -240,20 +261,17 @@ __global__ void __launch_bounds__(128) causal_conv_step_kernel(const T* __restri
   if (i >= batch * vectors) return;
   const int64_t b = i / vectors;
   const int c = (int)(i - b * vectors) * kV;
-  float win[kTaps][kV], f[kV];
+  constexpr int kP = PairsOf<kV>::n;
+  f2 win[kTaps][kP], f[kP];
 #pragma unroll
-  for (int k = 0; k < kTaps - 1; ++k) unpack<T, kV>(load<T, kV>(state + (b * (kTaps - 1) + k) * channels + c), win[k]);
-  unpack<T, kV>(load<T, kV>(x + b * xb + c), win[kTaps - 1]);
+  for (int k = 0; k < kTaps - 1; ++k) unpack2<T, kV>(load<T, kV>(state + (b * (kTaps - 1) + k) * channels + c), win[k]);
+  unpack2<T, kV>(load<T, kV>(x + b * xb + c), win[kTaps - 1]);
+  const Filter<kV, kTaps> filter(weight, bias, c);
 #pragma unroll
-  for (int q = 0; q < kV; ++q) {
-    float pre = bias != nullptr ? bias[c + q] : 0.0f;
+  for (int q = 0; q < kP; ++q) f[q] = activate2<kAct>(filter.at(win, q));
+  store2<T, kV>(y + b * channels + c, f);
 #pragma unroll
-    for (int k = 0; k < kTaps; ++k) pre = fmaf(weight[(c + q) * kTaps + k], win[k][q], pre);
-    f[q] = activate<kAct>(pre);
-  }
-  store<T, kV>(y + b * channels + c, f);
-#pragma unroll
-  for (int k = 0; k < kTaps - 1; ++k) store<T, kV>(state_out + (b * (kTaps - 1) + k) * channels + c, win[k + 1]);
+  for (int k = 0; k < kTaps - 1; ++k) store2<T, kV>(state_out + (b * (kTaps - 1) + k) * channels + c, win[k + 1]);
 }
 
 void plan(Conv* p, int v) {
@@ -263,7 +281,7 @@ void plan(Conv* p, int v) {
   p->runs = kThreads / p->lanes;
   p->vec_blocks = (vectors + p->lanes - 1) / p->lanes;
   // long runs read least twice; short ones fill the GPU
-  p->steps = 32;
+  p->steps = 64;
   while (p->steps > 4 && p->batch * p->vec_blocks * ((p->length + (int64_t)p->runs * p->steps - 1) / (p->runs * p->steps)) < 4 * sm_count())
     p->steps /= 2;
   p->time_blocks = (int)((p->length + (int64_t)p->runs * p->steps - 1) / (p->runs * p->steps));
@@ -296,13 +314,14 @@ int step(const void* x, int64_t xb, const void* state, void* state_out, void* y,
                    : (taps == 2 ? F<T, V, 2, kActNone>(__VA_ARGS__) : taps == 3 ? F<T, V, 3, kActNone>(__VA_ARGS__)    \
                                                                                 : F<T, V, 4, kActNone>(__VA_ARGS__)))
 #define ESGD_TYPE(F, ...)                                                                                             \
-  (is_bf16 ? (v == 8 ? ESGD_TAPS(__nv_bfloat16, 8, F, __VA_ARGS__) : ESGD_TAPS(__nv_bfloat16, 1, F, __VA_ARGS__))     \
+  (is_bf16 ? (v == 4 ? ESGD_TAPS(__nv_bfloat16, 4, F, __VA_ARGS__) : ESGD_TAPS(__nv_bfloat16, 1, F, __VA_ARGS__))     \
            : (v == 4 ? ESGD_TAPS(float, 4, F, __VA_ARGS__) : ESGD_TAPS(float, 1, F, __VA_ARGS__)))
 
 bool taken(int taps, int act) { return taps >= 2 && taps <= 4 && (act == kActSilu || act == kActNone); }
+// Channels of a thread: four where all rows begin on a multiple of four.
 int width(int is_bf16, int channels, int64_t xb, int64_t xt, const void* a, const void* b, const void* c, const void* d) {
-  const int v = is_bf16 ? 8 : 4;
-  return channels % v || xb % v || xt % v || !aligned16(a) || !aligned16(b) || !aligned16(c) || !aligned16(d) ? 1 : v;
+  const uintptr_t bytes = is_bf16 ? 8 : 16;
+  return channels % 4 || xb % 4 || xt % 4 || ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) % bytes ? 1 : 4;
 }
 
 }  // namespace
@@ -322,10 +341,10 @@ int esgd_causal_conv_fwd(const void* x, int64_t xb, int64_t xt, const void* stat
 }
 
 // The parts that esgd_causal_conv_bwd leaves in sums, each [channels * taps + channels].
-int64_t esgd_causal_conv_parts(int is_bf16, int64_t batch, int64_t length, int channels) {
+int64_t esgd_causal_conv_parts(int64_t batch, int64_t length, int channels) {
   // the narrowest vector has the most blocks of steps or fewer runs: room for either
   int64_t most = 0;
-  for (int v : {1, is_bf16 ? 8 : 4}) {
+  for (int v : {1, 4}) {
     if (channels % v) continue;
     Conv p = {batch, length, channels};
     plan(&p, v);

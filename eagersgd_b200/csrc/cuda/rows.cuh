@@ -21,17 +21,22 @@ template <> __device__ __forceinline__ __nv_bfloat16 as_type<__nv_bfloat16>(floa
 template <class T, int kV> struct Pack { T v[kV]; };
 template <> struct Pack<float, 4> { uint4 v; };
 template <> struct Pack<__nv_bfloat16, 8> { uint4 v; };
+template <> struct Pack<__nv_bfloat16, 4> { uint2 v; };
 
 template <class T, int kV> __device__ __forceinline__ Pack<T, kV> load(const T* p) {
-  static_assert(kV == 1 || kV * sizeof(T) == 16, "single elements or 16 bytes");
+  static_assert(kV == 1 || kV * sizeof(T) == 16 || kV * sizeof(T) == 8, "single elements, 8 or 16 bytes");
   Pack<T, kV> r;
   if constexpr (kV == 1) r.v[0] = *p;
+  else if constexpr (kV * sizeof(T) == 8) r.v = *reinterpret_cast<const uint2*>(p);
   else r.v = *reinterpret_cast<const uint4*>(p);
   return r;
 }
 template <class T, int kV> __device__ __forceinline__ void unpack(const Pack<T, kV>& r, float (&f)[kV]) {
   if constexpr (kV == 1) {
     f[0] = as_float(r.v[0]);
+  } else if constexpr (kV == 4 && sizeof(T) == 2) {
+    f[0] = __uint_as_float(r.v.x << 16); f[1] = __uint_as_float(r.v.x & 0xffff0000u);
+    f[2] = __uint_as_float(r.v.y << 16); f[3] = __uint_as_float(r.v.y & 0xffff0000u);
   } else if constexpr (kV == 4) {
     f[0] = __uint_as_float(r.v.x); f[1] = __uint_as_float(r.v.y); f[2] = __uint_as_float(r.v.z); f[3] = __uint_as_float(r.v.w);
   } else {
@@ -43,6 +48,9 @@ template <class T, int kV> __device__ __forceinline__ void unpack(const Pack<T, 
 template <class T, int kV> __device__ __forceinline__ void store(T* p, const float (&f)[kV]) {
   if constexpr (kV == 1) {
     *p = as_type<T>(f[0]);
+  } else if constexpr (kV == 4 && sizeof(T) == 2) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
   } else if constexpr (kV == 4) {
     *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
   } else {

@@ -739,37 +739,72 @@ __global__ void __launch_bounds__(256) selective_scan_narrow_kernel(const float*
 template <class T> __device__ __forceinline__ float at(const Seq& q, int64_t b, int c) {
   return as_float(reinterpret_cast<const T*>(q.p)[b * q.b + c]);
 }
+// Four states from the n-th on, as many as there are; kWhole: always four, on a boundary.
+template <class T, bool kWhole> __device__ __forceinline__ void four(const T* p, int n, int states, float (&to)[kStates]) {
+  if constexpr (kWhole) {
+    unpack<T, kStates>(load<T, kStates>(p + n), to);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kStates; ++j) to[j] = n + j < states ? as_float(p[n + j]) : 0.0f;
+  }
+}
 
-// One step of every sequence: the state moves on; state_out may be s.state.
-template <class T, int kLanes>
-__global__ void __launch_bounds__(kThreads) selective_scan_step_kernel(Scan s, float* state_out, T* __restrict__ out) {
+// One step of every sequence: the state moves on; state_out may be s.state.  A block has kWide channels of `many` sequences, one
+// after the other, each fetched while the one ahead is at work.  Bound by memory: 8 bytes a state.
+template <class T, int kLanes, bool kWhole>
+__global__ void __launch_bounds__(kThreads) selective_scan_step_kernel(Scan s, float* state_out, T* __restrict__ out, int many) {
   pdl_enter();
   constexpr int kWide = kThreads / kLanes;
   const int blocks = (s.channels + kWide - 1) / kWide;
-  const int64_t b = blockIdx.x / blocks;
-  const int c = (int)(blockIdx.x - b * blocks) * kWide + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-  const bool on = c < s.channels;
-  float part = 0.0f, u = 0.0f;
+  const int64_t rest = blockIdx.x / blocks, first = rest * many, last = first + many < s.batch ? first + many : s.batch;
+  const int c = (int)(blockIdx.x - rest * blocks) * kWide + threadIdx.x / kLanes, lane = threadIdx.x % kLanes, n = lane * kStates;
+  const bool on = c < s.channels && n < s.states;
+  float a[kStates] = {}, bias = 0.0f, skip = 0.0f;
   if (on) {
-    u = at<T>(s.u, b, c);
-    const float raw = at<T>(s.delta, b, c) + (s.bias != nullptr ? s.bias[c] : 0.0f);
-    const float dt = s.softplus ? softplus(raw) : raw;
+    four<float, kWhole>(s.A + (int64_t)c * s.states, n, s.states, a);
 #pragma unroll
-    for (int j = 0; j < kStates; ++j) {
-      const int n = lane * kStates + j;
-      if (n >= s.states) break;
-      const int64_t i = (b * s.channels + c) * s.states + n;
-      const float h = fmaf(exp2_approx(dt * (s.A[(int64_t)c * s.states + n] * kLog2e)), s.state[i], dt * u * at<T>(s.B, b, n));
-      state_out[i] = h;
-      part = fmaf(at<T>(s.C, b, n), h, part);
-    }
+    for (int j = 0; j < kStates; ++j) a[j] *= kLog2e;
+    if (s.bias != nullptr) bias = s.bias[c];
+    if (s.D != nullptr) skip = s.D[c];
   }
+  float h[kStates] = {}, bb[kStates] = {}, cc[kStates] = {}, u = 0.0f, delta = 0.0f, z = 0.0f;
+  auto fetch = [&](int64_t b) {
+    four<float, kWhole>(s.state + (b * s.channels + c) * s.states, n, s.states, h);
+    four<T, kWhole>(reinterpret_cast<const T*>(s.B.p) + b * s.B.b, n, s.states, bb);
+    four<T, kWhole>(reinterpret_cast<const T*>(s.C.p) + b * s.C.b, n, s.states, cc);
+    u = at<T>(s.u, b, c);
+    delta = at<T>(s.delta, b, c);
+    if (s.z.p != nullptr) z = at<T>(s.z, b, c);
+  };
+  if (on) fetch(first);
+  for (int64_t b = first; b < last; ++b) {
+    float part = 0.0f, x = 0.0f, gate = 0.0f, next[kStates];
+    if (on) {
+      const float raw = delta + bias, dt = s.softplus ? softplus(raw) : raw;
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-  if (on && lane == 0) {
-    if (s.D != nullptr) part = fmaf(s.D[c], u, part);
-    if (s.z.p != nullptr) part *= activate<kActSilu>(at<T>(s.z, b, c));
-    out[b * s.channels + c] = as_type<T>(part);
+      for (int j = 0; j < kStates; ++j) {
+        next[j] = fmaf(exp2_approx(dt * a[j]), h[j], dt * u * bb[j]);
+        part = fmaf(cc[j], next[j], part);
+      }
+      x = u;
+      gate = z;
+      if (b + 1 < last) fetch(b + 1);
+      float* to = state_out + (b * s.channels + c) * s.states + n;
+      if constexpr (kWhole) {
+        store<float, kStates>(to, next);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kStates; ++j)
+          if (n + j < s.states) to[j] = next[j];
+      }
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    if (on && lane == 0) {
+      part = fmaf(skip, x, part);
+      if (s.z.p != nullptr) part *= activate<kActSilu>(gate);
+      out[b * s.channels + c] = as_type<T>(part);
+    }
   }
 }
 
@@ -846,8 +881,16 @@ template <class T> int backward(const Scan& s, const Grads& g, void* dB, void* d
   }
 }
 template <class T, int kLanes> int step(const Scan& s, float* state_out, void* out, void* stream) {
-  return launch(selective_scan_step_kernel<T, kLanes>, dim3((unsigned)(s.batch * blocks_of(s.channels, kThreads / kLanes))), kThreads, 0, stream, s,
-                state_out, (T*)out);
+  // as many sequences to a block as leave eight blocks to every SM, four at most: A, D and the bias are read once for them
+  const int64_t blocks = blocks_of(s.channels, kThreads / kLanes);
+  int many = 1;
+  while (many < 4 && blocks * (s.batch / (2 * many)) >= 8 * sm_count()) many *= 2;
+  const dim3 grid((unsigned)((s.batch + many - 1) / many * blocks));
+  const uintptr_t bytes = 4 * sizeof(T);
+  const bool whole = s.states % 4 == 0 && aligned16(s.A) && aligned16(s.state) && aligned16(state_out) && (uintptr_t)s.B.p % bytes == 0 &&
+                     (uintptr_t)s.C.p % bytes == 0 && s.B.b % 4 == 0 && s.C.b % 4 == 0;
+  return whole ? launch(selective_scan_step_kernel<T, kLanes, true>, grid, kThreads, 0, stream, s, state_out, (T*)out, many)
+               : launch(selective_scan_step_kernel<T, kLanes, false>, grid, kThreads, 0, stream, s, state_out, (T*)out, many);
 }
 
 // F<T, kLanes>(...)

@@ -6,7 +6,7 @@ extern "C" {
 int esgd_causal_conv_fwd(const void* x, int64_t xb, int64_t xt, const void* state, const float* weight, const float* bias,
                          const int64_t* lengths, void* y, void* state_out, int is_bf16, int64_t batch, int64_t length, int channels, int taps,
                          int act, void* stream);
-int64_t esgd_causal_conv_parts(int is_bf16, int64_t batch, int64_t length, int channels);
+int64_t esgd_causal_conv_parts(int64_t batch, int64_t length, int channels);
 int esgd_causal_conv_bwd(const void* x, int64_t xb, int64_t xt, const void* state, const float* weight, const float* bias,
                          const int64_t* lengths, const void* dy, void* dx, float* sums, int64_t* parts, int is_bf16, int64_t batch,
                          int64_t length, int channels, int taps, int act, void* stream);
@@ -96,7 +96,7 @@ struct CausalConvFn : public Function<CausalConvFn> {
     Tensor dx, sums;
     if (need[0]) dx = at::empty({b, t, d}, x.options());
     const bool any = dw.out() != nullptr || db.out() != nullptr;
-    if (any) sums = at::empty({esgd_causal_conv_parts(is_bf16, b, t, (int)d), d * (taps + 1)}, f32);
+    if (any) sums = at::empty({esgd_causal_conv_parts(b, t, (int)d), d * (taps + 1)}, f32);
     int64_t parts = 0;
     ck(esgd_causal_conv_bwd(ptr(x), x.stride(0), x.stride(1), ptr(state), fptr(weight), fptr(bias), lengths_of(lengths), ptr(dy), mut(dx),
                             fptr(sums), &parts, is_bf16, b, t, (int)d, (int)taps, (int)ctx->saved_data["act"].toInt(), stream_of(x)),
