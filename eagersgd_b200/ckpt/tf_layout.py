@@ -42,6 +42,8 @@ def tf_variables(model: nn.Module, scope: str = "resnet_model") -> List[Tuple[st
             out += [(base + "gamma", mod.weight, "gamma"), (base + "beta", mod.bias, "beta"),
                     (base + "moving_mean", mod.running_mean, "mean"), (base + "moving_variance", mod.running_var, "var")]
             nbn += 1
+        elif kind == "gn":
+            raise NotImplementedError("the tf-models layout has no names for group norm; save the model's state_dict instead")
         elif kind == "dense":
             base = "%sdense%s/" % (pre, _suffix(ndense))
             out += [(base + "kernel", mod.weight, "dense_w"), (base + "bias", mod.bias, "dense_b")]

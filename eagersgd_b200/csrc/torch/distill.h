@@ -28,8 +28,8 @@ struct DistillFn : public Function<DistillFn> {
     const Tensor logits = aligned(logits_in.stride(1) == 1 && ld >= classes && ld < classes + 8 ? logits_in : logits_in.contiguous());
     const Tensor values = values_in.contiguous(), named = classes_in.contiguous(), labels = labels_in.defined() ? labels_in.contiguous() : Tensor();
     if (grad != nullptr) *grad = at::empty_strided({rows, classes}, {logits.stride(0), 1}, logits.options());
-    const auto f32 = logits.options().dtype(at::kFloat);
-    Tensor loss = at::empty({}, f32), row_loss = at::empty({rows}, f32);
+    Tensor loss = fresh_floats({}, logits);
+    const Tensor row_loss = fresh_floats({rows}, logits);
     ck(esgd_distill(ptr(logits), grad != nullptr ? mut(*grad) : nullptr, logits.scalar_type() == at::kBFloat16, ptr(values),
                     values.scalar_type() == at::kBFloat16, named.data_ptr<int64_t>(), labels.defined() ? labels.data_ptr<int64_t>() : nullptr,
                     (int)rows, (int)classes, (int)logits.stride(0), (int)top, (float)temperature, (float)hard_weight, fptr(row_loss), fptr(loss),

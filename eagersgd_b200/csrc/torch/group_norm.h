@@ -1,5 +1,6 @@
 // Group norm (+ residual) (+ activation) as an autograd operator; part of ops.cpp.
 #pragma once
+#include <ATen/cuda/EmptyTensor.h>
 
 extern "C" {
 int esgd_group_norm_max_group();
@@ -16,8 +17,16 @@ namespace {
 
 const void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* mut(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// at::empty without its way through the dispatcher: an operator's backward pass has up to ten of them, two microseconds each.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
+Tensor fresh_floats(at::IntArrayRef sizes, const Tensor& like) { return fresh(sizes, at::kFloat, like); }
+Tensor fresh_image(const Tensor& like) { return at::detail::empty_cuda(like.sizes(), like.scalar_type(), like.device(), kCL); }
 Tensor value_of(const c10::optional<Tensor>& o) { return o.has_value() ? *o : Tensor(); }
 bool differentiable(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+
+int64_t wants(const c10::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
 
 // bf16 or fp32.
 void check_float(const char* op, const char* name, const Tensor& t) {
@@ -50,8 +59,8 @@ void check_capture(const char* op, std::initializer_list<const Tensor*> tensors)
 struct ParamGrad {
   Sink sink;
   Tensor grad;
-  ParamGrad(AutogradContext* ctx, const char* key, bool wanted, at::IntArrayRef shape, at::TensorOptions f32) : sink(load_sink(ctx, key)) {
-    if (!sink && wanted) grad = at::empty(shape, f32);
+  ParamGrad(AutogradContext* ctx, const char* key, bool wanted, at::IntArrayRef shape, const Tensor& like) : sink(load_sink(ctx, key)) {
+    if (!sink && wanted) grad = fresh_floats(shape, like);
   }
   float* out() const { return sink ? sink->acc : fptr(grad); }
   int add() const { return sink ? 1 : 0; }
@@ -70,9 +79,7 @@ struct GroupNormFn : public Function<GroupNormFn> {
     ctx->save_for_backward({x, act != 0 ? res : Tensor(), gamma.t, beta.t, stats});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["act"] = act;
-    ctx->saved_data["need"] = std::vector<int64_t>{x_in.requires_grad(), gamma_in.has_value() && gamma_in->requires_grad(),
-                                                   beta_in.has_value() && beta_in->requires_grad(),
-                                                   res_in.has_value() && res_in->requires_grad()};
+    ctx->saved_data["need"] = (int64_t)x_in.requires_grad() | wants(gamma_in) << 1 | wants(beta_in) << 2 | wants(res_in) << 3;
     save_sink(ctx, "g", gs);
     save_sink(ctx, "b", bs);
     return z;
@@ -82,8 +89,8 @@ struct GroupNormFn : public Function<GroupNormFn> {
                     Tensor* stats) {
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t n = x.size(0), c = x.size(1), rows = x.size(2) * x.size(3);
-    Tensor z = empty_nhwc(n, c, x.size(2), x.size(3), x);
-    if (stats != nullptr) *stats = at::empty({n, groups, 2}, gamma.options());
+    Tensor z = fresh_image(x);
+    if (stats != nullptr) *stats = fresh_floats({n, groups, 2}, x);
     ck(esgd_group_norm_fwd(ptr(x), ptr(res), mut(z), fptr(gamma), fptr(beta), stats != nullptr ? fptr(*stats) : nullptr,
                            x.scalar_type() == at::kBFloat16, n, rows, (int)c, (int)groups, (int)act, (float)eps, stream_of(x)), "group_norm_act");
     return z;
@@ -93,16 +100,16 @@ struct GroupNormFn : public Function<GroupNormFn> {
     const Tensor &x = saved[0], &res = saved[1], &gamma = saved[2], &beta = saved[3], &stats = saved[4];
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t groups = ctx->saved_data["groups"].toInt(), act = ctx->saved_data["act"].toInt();
-    const auto need = ctx->saved_data["need"].toIntVector();
+    const int64_t need = ctx->saved_data["need"].toInt();
     const int64_t n = x.size(0), c = x.size(1), rows = x.size(2) * x.size(3);
     const Tensor dz = nhwc(grads[0]);
     Tensor dx, dres;
-    if (need[0]) dx = empty_nhwc(n, c, x.size(2), x.size(3), x);
-    if (need[3]) dres = act == 0 ? dz : empty_nhwc(n, c, x.size(2), x.size(3), x);
-    const ParamGrad dgamma(ctx, "g", need[1], {c}, gamma.options()), dbeta(ctx, "b", need[2], {c}, gamma.options());
+    if (need & 1) dx = fresh_image(x);
+    if (need & 8) dres = act == 0 ? dz : fresh_image(x);
+    const ParamGrad dgamma(ctx, "g", need & 2, {c}, x), dbeta(ctx, "b", need & 4, {c}, x);
     void* st = stream_of(x);
     const int64_t parts = rows > 0 ? n : 0;
-    Tensor sums = at::empty({parts, 2, c}, gamma.options());
+    const Tensor sums = fresh_floats({parts, 2, c}, x);
     ck(esgd_group_norm_bwd(ptr(x), ptr(res), ptr(dz), mut(dx), act == 0 ? nullptr : mut(dres), fptr(gamma), fptr(beta), fptr(stats), fptr(sums),
                            x.scalar_type() == at::kBFloat16, n, rows, (int)c, (int)groups, (int)act, st), "group_norm_act backward");
     ck(esgd_sum_parts(fptr(sums), parts, dbeta.out(), c, dbeta.add(), dgamma.out(), c, dgamma.add(), nullptr, 0, 0, st),

@@ -51,7 +51,7 @@ Tensor state_for(const char* op, const Opt& out, const Tensor& state) {
   TORCH_CHECK(a == b || a + state.nbytes() <= b || b + out->nbytes() <= a, op, ": out overlaps the state without being it");
   return *out;
 }
-Tensor room(int64_t floats, const at::TensorOptions& f32) { return floats > 0 ? at::empty({floats}, f32) : Tensor(); }
+Tensor room(int64_t floats, const Tensor& like) { return floats > 0 ? fresh_floats({floats}, like) : Tensor(); }
 void written(const Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 
 // ---------------------------------------------------------------- causal convolution
@@ -63,8 +63,7 @@ struct CausalConvFn : public Function<CausalConvFn> {
     variable_list out = run(x, weight.t, bias.t, state.t, lengths.t, act, want_state);
     ctx->save_for_backward({x, weight.t, bias.t, state.t, lengths.t});
     ctx->saved_data["act"] = act;
-    ctx->saved_data["need"] = std::vector<int64_t>{x_in.requires_grad(), weight_in.has_value() && weight_in->requires_grad(),
-                                                   bias_in.has_value() && bias_in->requires_grad()};
+    ctx->saved_data["need"] = (int64_t)x_in.requires_grad() | wants(weight_in) << 1 | wants(bias_in) << 2;
     save_sink(ctx, "w", ws);
     save_sink(ctx, "b", bs);
     if (want_state) ctx->mark_non_differentiable({out[1]});
@@ -74,8 +73,8 @@ struct CausalConvFn : public Function<CausalConvFn> {
                            bool want_state) {
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t b = x.size(0), t = x.size(1), d = x.size(2), taps = weight.size(1);
-    variable_list out = {at::empty({b, t, d}, x.options())};
-    if (want_state) out.push_back(at::empty({b, taps - 1, d}, x.options()));
+    variable_list out = {fresh({b, t, d}, x.scalar_type(), x)};
+    if (want_state) out.push_back(fresh({b, taps - 1, d}, x.scalar_type(), x));
     ck(esgd_causal_conv_fwd(ptr(x), x.stride(0), x.stride(1), ptr(state), fptr(weight), fptr(bias), lengths_of(lengths), mut(out[0]),
                             want_state ? mut(out[1]) : nullptr, x.scalar_type() == at::kBFloat16, b, t, (int)d, (int)taps, (int)act, stream_of(x)),
        "causal_conv");
@@ -87,16 +86,15 @@ struct CausalConvFn : public Function<CausalConvFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &state = saved[3], &lengths = saved[4];
     c10::cuda::CUDAGuard guard(x.device());
-    const auto need = ctx->saved_data["need"].toIntVector();
+    const int64_t need = ctx->saved_data["need"].toInt();
     const int64_t b = x.size(0), t = x.size(1), d = x.size(2), taps = weight.size(1);
     const bool is_bf16 = x.scalar_type() == at::kBFloat16;
-    const auto f32 = weight.options();
     const Tensor dy = dense(grads[0]);
-    const ParamGrad dw(ctx, "w", need[1], {d, taps}, f32), db(ctx, "b", need[2], {d}, f32);
+    const ParamGrad dw(ctx, "w", need & 2, {d, taps}, x), db(ctx, "b", need & 4, {d}, x);
     Tensor dx, sums;
-    if (need[0]) dx = at::empty({b, t, d}, x.options());
+    if (need & 1) dx = fresh({b, t, d}, x.scalar_type(), x);
     const bool any = dw.out() != nullptr || db.out() != nullptr;
-    if (any) sums = at::empty({esgd_causal_conv_parts(b, t, (int)d), d * (taps + 1)}, f32);
+    if (any) sums = fresh_floats({esgd_causal_conv_parts(b, t, (int)d), d * (taps + 1)}, x);
     int64_t parts = 0;
     ck(esgd_causal_conv_bwd(ptr(x), x.stride(0), x.stride(1), ptr(state), fptr(weight), fptr(bias), lengths_of(lengths), ptr(dy), mut(dx),
                             fptr(sums), &parts, is_bf16, b, t, (int)d, (int)taps, (int)ctx->saved_data["act"].toInt(), stream_of(x)),
@@ -158,7 +156,7 @@ std::pair<Tensor, Tensor> causal_conv_step(const Tensor& x_in, const Tensor& sta
   const Tensor x = rows_dense(x_in);
   const int64_t b = x.size(0), d = x.size(1);
   TORCH_CHECK(b * d < ((int64_t)1 << 37), op, ": an input of ", x.sizes(), " is too large");
-  Tensor y = at::empty({b, d}, x.options());
+  Tensor y = fresh({b, d}, x.scalar_type(), x);
   ck(esgd_causal_conv_step(ptr(x), x.stride(0), ptr(state), mut(next), fptr(weight), fptr(value_of(bias)), mut(y),
                            x.scalar_type() == at::kBFloat16, b, (int)d, (int)weight.size(1), (int)act, stream_of(x)), op);
   written(next);
@@ -204,8 +202,7 @@ struct SelectiveScanFn : public Function<SelectiveScanFn> {
     variable_list out = run(in, want_state, &keep);
     ctx->save_for_backward({in.u, in.delta, in.z, in.B, in.C, A.t, D.t, bias.t, lengths.t, keep});
     ctx->saved_data["softplus"] = softplus;
-    ctx->saved_data["need"] = std::vector<int64_t>{A_in.has_value() && A_in->requires_grad(), D_in.has_value() && D_in->requires_grad(),
-                                                   bias_in.has_value() && bias_in->requires_grad()};
+    ctx->saved_data["need"] = wants(A_in) | wants(D_in) << 1 | wants(bias_in) << 2;
     save_sink(ctx, "A", as);
     save_sink(ctx, "D", ds);
     save_sink(ctx, "b", bs);
@@ -215,10 +212,10 @@ struct SelectiveScanFn : public Function<SelectiveScanFn> {
   static variable_list run(const ScanInputs& in, bool want_state, Tensor* keep) {
     c10::cuda::CUDAGuard guard(in.u.device());
     const esgd_scan e = in.args();
-    variable_list out = {at::empty(in.u.sizes(), in.u.options())};
-    if (want_state) out.push_back(at::empty({e.batch, e.channels, e.states}, in.A.options()));
-    if (keep != nullptr) *keep = at::empty({esgd_selective_scan_keep(&e)}, in.A.options());
-    const Tensor local = room(esgd_selective_scan_local(&e, 0), in.A.options());
+    variable_list out = {fresh(in.u.sizes(), in.u.scalar_type(), in.u)};
+    if (want_state) out.push_back(fresh_floats({e.batch, e.channels, e.states}, in.u));
+    if (keep != nullptr) *keep = fresh_floats({esgd_selective_scan_keep(&e)}, in.u);
+    const Tensor local = room(esgd_selective_scan_local(&e, 0), in.u);
     ck(esgd_selective_scan_fwd(&e, mut(out[0]), want_state ? fptr(out[1]) : nullptr, keep != nullptr ? fptr(*keep) : nullptr, fptr(local),
                                stream_of(in.u)), "selective_scan");
     return out;
@@ -232,19 +229,20 @@ struct SelectiveScanFn : public Function<SelectiveScanFn> {
     const Tensor& keep = saved[9];
     c10::cuda::CUDAGuard guard(in.u.device());
     const esgd_scan e = in.args();
-    const auto need = ctx->saved_data["need"].toIntVector();
-    const auto f32 = in.A.options();
+    const int64_t need = ctx->saved_data["need"].toInt();
     const int64_t d = e.channels, n = e.states;
+    const auto type = in.u.scalar_type();
     const Tensor dout = dense(grads[0]);
-    Tensor du = at::empty(in.u.sizes(), in.u.options()), ddelta = at::empty_like(du), dz = in.z.defined() ? at::empty_like(du) : Tensor();
-    Tensor dB = at::empty({e.batch, e.length, n}, in.u.options()), dC = at::empty_like(dB);
-    const ParamGrad dA(ctx, "A", need[0], {d, n}, f32), dD(ctx, "D", need[1], {d}, f32), db(ctx, "b", need[2], {d}, f32);
-    const int64_t parts = esgd_selective_scan_parts(&e);
-    const Tensor narrow = at::empty({esgd_selective_scan_narrow(&e)}, f32), sums = at::empty({parts, d * (n + 2)}, f32);
-    const Tensor local = room(esgd_selective_scan_local(&e, 1), f32);
-    ck(esgd_selective_scan_bwd(&e, ptr(dout), fptr(keep), mut(du), mut(ddelta), mut(dz), mut(dB), mut(dC), fptr(narrow), fptr(sums),
-                               fptr(local), stream_of(in.u)), "selective_scan backward");
-    ck(esgd_sum_parts(fptr(sums), parts, dA.out(), d * n, dA.add(), dD.out(), d, dD.add(), db.out(), d, db.add(), stream_of(in.u)),
+    Tensor du = fresh(in.u.sizes(), type, in.u), ddelta = fresh(in.u.sizes(), type, in.u), dz = in.z.defined() ? fresh(in.u.sizes(), type, in.u) : Tensor();
+    Tensor dB = fresh({e.batch, e.length, n}, type, in.u), dC = fresh({e.batch, e.length, n}, type, in.u);
+    const ParamGrad dA(ctx, "A", need & 1, {d, n}, in.u), dD(ctx, "D", need & 2, {d}, in.u), db(ctx, "b", need & 4, {d}, in.u);
+    // one workspace: the shares of dB and dC, those of the parameters, and the chunks' states; each on 16 bytes
+    const int64_t parts = esgd_selective_scan_parts(&e), n_narrow = esgd_selective_scan_narrow(&e), n_sums = (parts * d * (n + 2) + 3) / 4 * 4;
+    const Tensor work = room(n_narrow + n_sums + esgd_selective_scan_local(&e, 1), in.u);
+    float *narrow = fptr(work), *sums = narrow + n_narrow, *local = sums + n_sums;
+    ck(esgd_selective_scan_bwd(&e, ptr(dout), fptr(keep), mut(du), mut(ddelta), mut(dz), mut(dB), mut(dC), narrow, sums, local,
+                               stream_of(in.u)), "selective_scan backward");
+    ck(esgd_sum_parts(sums, parts, dA.out(), d * n, dA.add(), dD.out(), d, dD.add(), db.out(), d, db.add(), stream_of(in.u)),
        "selective_scan parameter gradients");
     dA.done();
     dD.done();
@@ -319,7 +317,7 @@ std::pair<Tensor, Tensor> selective_scan_step(const Tensor& u, const Tensor& del
   const ScanInputs in = {rows_dense(u), rows_dense(delta), z.has_value() ? rows_dense(*z) : Tensor(), rows_dense(B), rows_dense(C), A,
                          value_of(D), value_of(bias), state, Tensor(), softplus};
   const esgd_scan e = in.args();
-  Tensor y = at::empty(u.sizes(), u.options());
+  Tensor y = fresh(u.sizes(), u.scalar_type(), u);
   ck(esgd_selective_scan_step(&e, fptr(next), mut(y), stream_of(u)), op);
   written(next);
   return {y, next};

@@ -1,12 +1,14 @@
-"""Model zoo: ResNets (CIFAR / ImageNet), LSTM classifier, hyperplane regressor, small nets."""
+"""Model zoo: ResNets (CIFAR / ImageNet), LSTM and scan classifiers, hyperplane regressor, small nets."""
 from .resnet import ResNet, cifar_resnet, imagenet_resnet, count_parameters  # noqa: F401
 from .hyperplane import HyperplaneRegressor, HyperplaneData  # noqa: F401
 from .lstm import LSTMClassifier  # noqa: F401
+from .scan import ScanClassifier  # noqa: F401
 from .small import MnistNet, SimpleCNN, DeepMnistNet, WideResNet  # noqa: F401
 
 _FACTORIES = {
     "simple_mnist": lambda **kw: MnistNet(**kw), "simple_cnn": lambda **kw: SimpleCNN(**kw), "deep_mnist": lambda **kw: DeepMnistNet(**kw),
     "wide_resnet": lambda **kw: WideResNet(**kw), "lstm": lambda **kw: LSTMClassifier(**kw),
+    "scan": lambda **kw: ScanClassifier(**kw),
     "hyperplane": lambda **kw: HyperplaneRegressor(**kw),
 }
 
@@ -26,7 +28,7 @@ def create_model(name: str, *args, **kw):
     if name not in _FACTORIES:
         raise KeyError("unknown model %r (known: resnet, %s)" % (name, ", ".join(sorted(_FACTORIES))))
     if classes is not None and name not in ("hyperplane",):
-        kw.setdefault("num_classes" if name == "lstm" else "classes", classes)
+        kw.setdefault("num_classes" if name in ("lstm", "scan") else "classes", classes)
     if shape is not None and name == "simple_cnn":
         kw.setdefault("in_channels", shape[0])
         kw.setdefault("size", shape[1])

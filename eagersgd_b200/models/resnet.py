@@ -51,11 +51,27 @@ class BatchNormAct(nn.BatchNorm2d):
                           residual, stats, self.training)
 
 
-def _bn(ch: int, zero_gamma: bool = False) -> BatchNormAct:
-    bn = BatchNormAct(ch, eps=BN_EPS, momentum=1.0 - BN_MOMENTUM_TF)
+class GroupNormAct(nn.GroupNorm):
+    """Group norm in the place of ``BatchNormAct``: no statistics of the batch, so replicas that see other samples, or miss a
+    round, compute the same function, and a batch of one is as good as any."""
+
+    def forward(self, y, relu: bool = True, residual=None, stats=None):  # noqa: D102
+        return ops.group_norm_act(y, self.num_groups, self.weight, self.bias, "relu" if relu else None, residual, self.eps)
+
+
+NORM_GROUPS = 32
+
+
+def _norm(norm: str, ch: int, zero_gamma: bool = False) -> nn.Module:
+    """``group``: 32 groups at most, of eight channels or more."""
+    if norm == "group":
+        groups = max(g for g in range(1, NORM_GROUPS + 1) if ch % g == 0 and (ch // g >= 8 or g == 1))
+        m = GroupNormAct(groups, ch, eps=BN_EPS)
+    else:
+        m = BatchNormAct(ch, eps=BN_EPS, momentum=1.0 - BN_MOMENTUM_TF)
     if zero_gamma:
-        nn.init.zeros_(bn.weight)
-    return bn
+        nn.init.zeros_(m.weight)
+    return m
 
 
 class _Conv(nn.Conv2d):
@@ -65,13 +81,14 @@ class _Conv(nn.Conv2d):
     squares of ``y`` when the kernel produced them in its epilogue (else ``None``).
     """
 
-    def __init__(self, cin, cout, k, stride):
+    def __init__(self, cin, cout, k, stride, statistics=True):
         super().__init__(cin, cout, k, stride=stride, padding=(k - 1) // 2, bias=False)
+        self.statistics = statistics         # whether a batch norm follows, which uses them
         # variance_scaling_initializer() of the reference: fan-in scaling
         nn.init.kaiming_normal_(self.weight, mode="fan_in", nonlinearity="linear")
 
     def forward(self, x, tap_input: bool = False):  # noqa: D102
-        return ops.conv2d(x, self.weight, self.stride[0], self.padding[0], want_stats=self.training,
+        return ops.conv2d(x, self.weight, self.stride[0], self.padding[0], want_stats=self.training and self.statistics,
                           tap_input=tap_input)
 
 
@@ -92,34 +109,35 @@ def _train_layer(conv, bn):
 
 
 class _Block(nn.Module):
-    def __init__(self, cin, filters, stride, kind, version, project, registry):
+    def __init__(self, cin, filters, stride, kind, version, project, registry, norm="batch"):
         super().__init__()
         self.kind, self.version = kind, version
+        tag, batch = "bn" if norm == "batch" else "gn", norm == "batch"
         cout = filters * 4 if kind == "bottleneck" else filters
         self.proj = self.proj_bn = None
         if version == 2:
-            self.pre_bn = _bn(cin)
-            registry.append(("bn", self.pre_bn))
+            self.pre_bn = _norm(norm, cin)
+            registry.append((tag, self.pre_bn))
         if project:
-            self.proj = _Conv(cin, cout, 1, stride)
+            self.proj = _Conv(cin, cout, 1, stride, batch)
             registry.append(("conv", self.proj))
             if version == 1:
-                self.proj_bn = _bn(cout)
-                registry.append(("bn", self.proj_bn))
+                self.proj_bn = _norm(norm, cout)
+                registry.append((tag, self.proj_bn))
         convs, bns = [], []
         if kind == "bottleneck":
             spec = [(cin, filters, 1, 1), (filters, filters, 3, stride), (filters, cout, 1, 1)]
         else:
             spec = [(cin, filters, 3, stride), (filters, filters, 3, 1)]
         for idx, (ci, co, k, s) in enumerate(spec):
-            conv = _Conv(ci, co, k, s)
+            conv = _Conv(ci, co, k, s, batch)
             convs.append(conv)
             registry.append(("conv", conv))
             last = idx == len(spec) - 1
             if version == 1 or not last:
-                bn = _bn(co, zero_gamma=(last and version == 1))
+                bn = _norm(norm, co, zero_gamma=(last and version == 1))
                 bns.append(bn)
-                registry.append(("bn", bn))
+                registry.append((tag, bn))
         self.convs = nn.ModuleList(convs)
         self.bns = nn.ModuleList(bns)
         self.cout = cout
@@ -167,31 +185,34 @@ class _Block(nn.Module):
 
 class ResNet(nn.Module):
     def __init__(self, kind: str, blocks: List[int], num_classes: int, num_filters: int, first_kernel: int,
-                 first_stride: int, first_pool: bool, block_strides: List[int], version: int = 1):
+                 first_stride: int, first_pool: bool, block_strides: List[int], version: int = 1, norm: str = "batch"):
         super().__init__()
         assert version in (1, 2)
-        self.version = version
+        if norm not in ("batch", "group"):
+            raise ValueError("norm is 'batch' or 'group', not %r" % (norm,))
+        self.version, self.norm = version, norm
+        tag = "bn" if norm == "batch" else "gn"
         self.registry: List[Tuple[str, nn.Module]] = []  # creation order, for the tf-models variable names
-        self.stem = _Conv(3, num_filters, first_kernel, first_stride)
+        self.stem = _Conv(3, num_filters, first_kernel, first_stride, norm == "batch")
         self.registry.append(("conv", self.stem))
         self.stem_bn = None
         if version == 1:
-            self.stem_bn = _bn(num_filters)
-            self.registry.append(("bn", self.stem_bn))
+            self.stem_bn = _norm(norm, num_filters)
+            self.registry.append((tag, self.stem_bn))
         self.first_pool = first_pool
         layers = []
         cin = num_filters
         for i, nb in enumerate(blocks):
             filters = num_filters * (2 ** i)
             for j in range(nb):
-                blk = _Block(cin, filters, block_strides[i] if j == 0 else 1, kind, version, j == 0, self.registry)
+                blk = _Block(cin, filters, block_strides[i] if j == 0 else 1, kind, version, j == 0, self.registry, norm)
                 layers.append(blk)
                 cin = blk.cout
         self.blocks = nn.ModuleList(layers)
         self.final_bn = None
         if version == 2:
-            self.final_bn = _bn(cin)
-            self.registry.append(("bn", self.final_bn))
+            self.final_bn = _norm(norm, cin)
+            self.registry.append((tag, self.final_bn))
         self.fc = nn.Linear(cin, num_classes)
         self.registry.append(("dense", self.fc))
         self.feature_dim = cin
@@ -219,7 +240,7 @@ class ResNet(nn.Module):
         """The coefficients of the network's batch norms by module, when the fused inference path applies: no gradients,
         every layer in evaluation mode and what it was built as, and nobody listening to a layer's output; else None.  Asked
         in every pass: a layer may have been exchanged, parametrized or hooked since the last one."""
-        if self.training or torch.is_grad_enabled() or not ops.native(x) or nn.modules.module._has_any_global_hook():
+        if self.norm != "batch" or self.training or torch.is_grad_enabled() or not ops.native(x) or nn.modules.module._has_any_global_hook():
             return None
         st = _eval_state.setdefault(self, {})
         for renewed in (False, True):
@@ -294,19 +315,19 @@ class ResNet(nn.Module):
         return ops.linear(self.features(x), self.fc.weight, self.fc.bias)
 
 
-def imagenet_resnet(size: int = 50, version: int = 1, num_classes: int = 1001) -> ResNet:
+def imagenet_resnet(size: int = 50, version: int = 1, num_classes: int = 1001, norm: str = "batch") -> ResNet:
     """ImagenetModel (imagenet_main_eagersgd.py:290-330).  ``version=1`` is the
-    reference's v1 with the stride on the 3x3 convolution, i.e. "ResNet v1.5"."""
+    reference's v1 with the stride on the 3x3 convolution, i.e. "ResNet v1.5".  ``norm="group"``: group norm instead of batch norm."""
     kind, blocks = IMAGENET_BLOCKS[size]
-    return ResNet(kind, blocks, num_classes, 64, 7, 2, True, [1, 2, 2, 2], version)
+    return ResNet(kind, blocks, num_classes, 64, 7, 2, True, [1, 2, 2, 2], version, norm)
 
 
-def cifar_resnet(size: int = 32, version: int = 1, num_classes: int = 10) -> ResNet:
+def cifar_resnet(size: int = 32, version: int = 1, num_classes: int = 10, norm: str = "batch") -> ResNet:
     """Cifar10Model: 6n+2 layers, 16/32/64 filters, building blocks (cifar10_main.py:179-219)."""
     if size % 6 != 2:
         raise ValueError("resnet_size must be 6n + 2")
     n = (size - 2) // 6
-    return ResNet("building", [n] * 3, num_classes, 16, 3, 1, False, [1, 2, 2], version)
+    return ResNet("building", [n] * 3, num_classes, 16, 3, 1, False, [1, 2, 2], version, norm)
 
 
 def count_parameters(model: nn.Module) -> Tuple[int, int]:

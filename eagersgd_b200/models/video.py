@@ -16,18 +16,25 @@ import torch.nn as nn
 from ..ops import functional as ops
 from .lstm import LSTMClassifier
 from .resnet import imagenet_resnet
+from .scan import ScanClassifier
 
 
 class ResNetLSTM(nn.Module):
     def __init__(self, num_classes: int = 101, resnet_size: int = 50, hidden: int = 256, layers: int = 2,
-                 dropout: float = 0.5, frame_chunk: int = 64, frame_net: nn.Module = None, feature_dim: int = None):
+                 dropout: float = 0.5, frame_chunk: int = 64, frame_net: nn.Module = None, feature_dim: int = None,
+                 sequence: str = "lstm", norm: str = "batch"):
+        """``sequence="scan"``: selective scans over the frames instead of the LSTM; ``norm="group"``: group norm in the frame network,
+        whose batch is the frames of all clips."""
         super().__init__()
-        self.frame_net = frame_net if frame_net is not None else imagenet_resnet(resnet_size, 1, 1000)
+        if sequence not in ("lstm", "scan"):
+            raise ValueError("sequence is 'lstm' or 'scan', not %r" % (sequence,))
+        self.frame_net = frame_net if frame_net is not None else imagenet_resnet(resnet_size, 1, 1000, norm)
         if feature_dim is None:
             feature_dim = self.frame_net.fc.in_features
         self.feature_dim, self.frame_chunk = feature_dim, frame_chunk
         # the LSTM stack of the sequence classifier, with a head applied at every time step instead of the last
-        self.rnn = LSTMClassifier(feature_dim, hidden, layers, num_classes, dropout=dropout)
+        self.rnn = LSTMClassifier(feature_dim, hidden, layers, num_classes, dropout=dropout) if sequence == "lstm" else \
+            ScanClassifier(feature_dim, hidden, layers, num_classes)
 
     def compute_dtype_(self, dtype):
         self.rnn.compute_dtype_(dtype)

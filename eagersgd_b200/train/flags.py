@@ -81,6 +81,8 @@ def define_resnet(p, default_size=50, sizes=(18, 34, 50, 101, 152, 200)):
     g.add_argument("--imbalance_seconds", type=float, default=0.32)
     g.add_argument("--batchaug", type=int, default=1)
     g.add_argument("--virtual_batch_size", type=int, default=None)
+    g.add_argument("--norm", default="batch", choices=["batch", "group"],
+                   help="group: group norm instead of batch norm (no statistics of the batch, which replicas do not share)")
 
 
 def build_parser(description: str, default_size: int = 50) -> argparse.ArgumentParser:

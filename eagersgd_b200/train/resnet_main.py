@@ -53,8 +53,8 @@ DATASETS = {
 
 def build_model(args, info):
     if args.dataset == "imagenet":
-        return imagenet_resnet(args.resnet_size, args.resnet_version, info["classes"])
-    return cifar_resnet(args.resnet_size, args.resnet_version, info["classes"])
+        return imagenet_resnet(args.resnet_size, args.resnet_version, info["classes"], args.norm)
+    return cifar_resnet(args.resnet_size, args.resnet_version, info["classes"], args.norm)
 
 
 def build_data(args, info, group):
