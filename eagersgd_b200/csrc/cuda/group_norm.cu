@@ -453,9 +453,11 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
   if (s.split > 1) cluster.barrier_wait();        // nobody leaves while its sums are being read
 }
 
-// A slice has whole groups and whole vectors, and 128 bytes or more of a row where it can, so that a warp reads whole lines (more where
-// a slice of so few pixels is hardly worth a CTA, as long as all SMs have some); a cluster has as many CTAs as keep two of them busy on every SM with eight rows a thread or more, and its rows in shared memory:
-// `budget` bytes a CTA for `tensors` of them.  False where a slice is too wide.
+// A slice has whole groups and whole vectors, and 128 bytes or more of a row where it can, so that a warp reads whole lines; more where
+// a slice of so few pixels is hardly worth a CTA, as long as all SMs have some (256x512x7x7: 27 -> 17 us forward).  A cluster has as
+// many CTAs as give three to every two SMs, and up to four so that its rows stay in shared memory, `budget` bytes a CTA for
+// `tensors` of them: 128x256x56x56 with residual forward / backward 180 / 321 us with two, 161 / 308 with four, 181 / 320 with eight.
+// False where a slice is too wide.
 constexpr int kSmallUnit = 16 * 1024;
 bool plan(int64_t samples, int64_t rows, int channels, int groups, int v, int size, int tensors, int budget, Shape* s) {
   s->rows = rows;
@@ -471,7 +473,9 @@ bool plan(int64_t samples, int64_t rows, int channels, int groups, int v, int si
   const int64_t units = samples * (channels / s->slice), row = (int64_t)s->slice * size * tensors;
   const int lanes = kThreads / (s->slice / v < kThreads ? s->slice / v : kThreads);
   s->split = 1;
-  while (s->split < 8 && rows / s->split >= 8 * lanes && (units * s->split < 2 * sm_count() || rows / s->split * row > budget)) s->split *= 2;
+  while (s->split < 8 && rows / s->split >= 8 * lanes &&
+         (2 * units * s->split < 3 * sm_count() || (s->split < 4 && rows / s->split * row > budget)))
+    s->split *= 2;
   const int64_t held = v > 1 ? budget / row : 0, most = (rows + s->split - 1) / s->split;
   s->held = (int)(held < most ? held : most);
   return true;
