@@ -182,6 +182,7 @@ __device__ __forceinline__ int left_of(int width, int c) { return width - c < 0 
 
 // Forward passes.  A row of partial sums: a warp's channels of every lane fall into banks of their own.
 template <int kLanes> struct Lanes : Share<kTile, 2 * kThreads / kLanes, kLanes * kStates> {
+  static_assert(kLanes <= kTile, "every thread's pairs are steps of the tile");
   static constexpr int kRow = 2 * kThreads / kLanes + (32 / kLanes - 2 * kThreads / kLanes % 32 + 32) % 32;
 };
 
@@ -261,10 +262,10 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
   const ulonglong2* dt2 = reinterpret_cast<const ulonglong2*>(s_dt) + c / 2;
   float* put_y = s_y + lane * In::kRow + c;
   for (int64_t t0 = p.first; t0 < p.last; t0 += kTile) {
+    // Steps behind the end are prepared as well, out of whatever is there, and not used: without branches the pairs' chains overlap.
     float2 du[In::kPairs], gate[In::kPairs];             // D u and silu(z) of the tile, for its end
 #pragma unroll
     for (int k = 0; k < In::kPairs; ++k) {
-      if (in.step + k * In::kPitch >= steps) continue;
       const float2 uv = u[k].get(), dv = delta[k].get();
       const float x = dv.x + bias.x, w = dv.y + bias.y;
       const float tx = s.softplus ? softplus(x) : x, tw = s.softplus ? softplus(w) : w;
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
     }
 #pragma unroll
     for (int k = 0; k < In::kNarrow; ++k) {
-      if (in.narrow_step + k * In::kNarrowPitch >= steps) continue;
+      if (In::kNarrowPitch > kTile && in.narrow_step >= kTile) continue;
       *reinterpret_cast<float2*>(put_bc + k * In::kNarrowPitch * 2 * kPadded) = bb[k].get();
       *reinterpret_cast<float2*>(put_bc + k * In::kNarrowPitch * 2 * kPadded + kStates) = cc[k].get();
     }
@@ -315,7 +316,6 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < In::kPairs; ++k) {
-      if (in.step + k * In::kPitch >= now) continue;
       float v = 0.0f, w = 0.0f;
 #pragma unroll
       for (int l = 0; l < kLanes; ++l) {
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
         v += part.x;
         w += part.y;
       }
-      put<T, kEven>(y + k * y_pitch, two, (v + du[k].x) * gate[k].x, (w + du[k].y) * gate[k].y);
+      put<T, kEven>(y + k * y_pitch, in.step + k * In::kPitch < now ? two : 0, (v + du[k].x) * gate[k].x, (w + du[k].y) * gate[k].y);
     }
     y += (int64_t)kTile * s.channels;
   }
@@ -390,7 +390,6 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
     if (i > 0) __syncthreads();
 #pragma unroll
     for (int k = 0; k < In::kPairs; ++k) {
-      if (in.step + k * In::kPitch >= steps) continue;
       float2 v = x[k].get();
       const float2 dv = delta[k].get();
       const float e = dv.x + bias.x, w = dv.y + bias.y;
@@ -409,7 +408,8 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
     }
 #pragma unroll
     for (int k = 0; k < In::kNarrow; ++k)
-      if (in.narrow_step + k * In::kNarrowPitch < steps) *reinterpret_cast<float2*>(put_bc + k * In::kNarrowPitch * kPadded) = bc[k].get();
+      if (In::kNarrowPitch <= kTile || in.narrow_step < kTile)
+        *reinterpret_cast<float2*>(put_bc + k * In::kNarrowPitch * kPadded) = bc[k].get();
     __syncthreads();
     const int now = steps;
     const int64_t after = p.first + (kReverse ? tiles - 2 - i : i + 1) * kTile;
