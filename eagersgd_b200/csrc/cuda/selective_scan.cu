@@ -268,14 +268,11 @@ __global__ void __launch_bounds__(kThreads) selective_scan_fwd_kernel(Scan s, T*
     for (int k = 0; k < In::kPairs; ++k) {
       const float2 uv = u[k].get(), dv = delta[k].get();
       const float x = dv.x + bias.x, w = dv.y + bias.y;
-      const float tx = s.softplus ? softplus(x) : x, tw = s.softplus ? softplus(w) : w;
+      const float px = softplus(x), pw = softplus(w), tx = s.softplus ? px : x, tw = s.softplus ? pw : w;
       put_dt[k * In::kPitch * kWide / 2] = make_float4(tx, tw, tx * uv.x, tw * uv.y);
       du[k] = make_float2(skip.x * uv.x, skip.y * uv.y);
-      gate[k] = make_float2(1.0f, 1.0f);
-      if (gated) {
-        const float2 zv = z[k].get();
-        gate[k] = make_float2(activate<kActSilu>(zv.x), activate<kActSilu>(zv.y));
-      }
+      const float2 zv = z[k].get(), silu = make_float2(activate<kActSilu>(zv.x), activate<kActSilu>(zv.y));
+      gate[k] = make_float2(gated ? silu.x : 1.0f, gated ? silu.y : 1.0f);
     }
 #pragma unroll
     for (int k = 0; k < In::kNarrow; ++k) {
@@ -393,13 +390,11 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
       float2 v = x[k].get();
       const float2 dv = delta[k].get();
       const float e = dv.x + bias.x, w = dv.y + bias.y;
-      const float te = s.softplus ? softplus(e) : e, tw = s.softplus ? softplus(w) : w;
+      const float pe = softplus(e), pw = softplus(w), te = s.softplus ? pe : e, tw = s.softplus ? pw : w;
       if constexpr (kReverse) {
-        if (gated) {
-          const float2 zv = z[k].get();
-          v.x *= activate<kActSilu>(zv.x);
-          v.y *= activate<kActSilu>(zv.y);
-        }
+        const float2 zv = z[k].get(), silu = make_float2(activate<kActSilu>(zv.x), activate<kActSilu>(zv.y));
+        v.x *= gated ? silu.x : 1.0f;
+        v.y *= gated ? silu.y : 1.0f;
       } else {
         v.x *= te;
         v.y *= tw;
@@ -574,16 +569,13 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
         const float2 dv = delta[0].get(), ov = up[0].get();
         uv = u[0].get();
         const float x = dv.x + bias.x, w = dv.y + bias.y;
-        dt = make_float2(x, w);
-        slope_dt = make_float2(1.0f, 1.0f);
-        if (s.softplus) dt = make_float2(softplus(x, &slope_dt.x), softplus(w, &slope_dt.y));
-        dy = ov;
-        if (gated) {
-          const float2 zv = z[0].get();
-          const float gx = sigmoid(zv.x), gw = sigmoid(zv.y);
-          dy = make_float2(ov.x * zv.x * gx, ov.y * zv.y * gw);
-          dz = make_float2(ov.x * gx * (1.0f + zv.x * (1.0f - gx)), ov.y * gw * (1.0f + zv.y * (1.0f - gw)));
-        }
+        const float px = softplus(x, &slope_dt.x), pw = softplus(w, &slope_dt.y);
+        dt = make_float2(s.softplus ? px : x, s.softplus ? pw : w);
+        slope_dt = make_float2(s.softplus ? slope_dt.x : 1.0f, s.softplus ? slope_dt.y : 1.0f);
+        const float2 zv = z[0].get();
+        const float gx = sigmoid(zv.x), gw = sigmoid(zv.y);
+        dy = make_float2(gated ? ov.x * zv.x * gx : ov.x, gated ? ov.y * zv.y * gw : ov.y);
+        dz = make_float2(ov.x * gx * (1.0f + zv.x * (1.0f - gx)), ov.y * gw * (1.0f + zv.y * (1.0f - gw)));
       }
       s_dt[in.step][in.channel / 2] = make_float4(dt.x, dt.y, dt.x * uv.x, dt.y * uv.y);
       s_dy[in.step][in.channel / 2] = pair(dy);
