@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 2) causal_conv_bwd_kernel(const T* _
                                                                       Conv p) {
   pdl_enter();
   constexpr int kP = PairsOf<kV>::n;
-  __shared__ float stage[(kTaps + 1) * kThreads * kV];
+  __shared__ __align__(16) float stage[(kTaps + 1) * kThreads * kV];
   const Spot<kV> s(p);
   f2 dw[kTaps + 1][kP];
 #pragma unroll

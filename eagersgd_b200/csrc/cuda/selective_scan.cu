@@ -460,7 +460,8 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-// d += a b with eleven bits of each factor, or (fp32 gradients) with the next eleven as well.
+// d += a b with eleven bits of each factor, or (fp32 gradients) with the next eleven as well.  A step's column is its own, the others of
+// the product are times zero: a state that is no number, or infinite, makes dB and dC of all eight steps of its tile no numbers.
 // bh: the rounded factor.
 template <bool kFine>
 __device__ __forceinline__ void product(float (&d)[4], const float (&a)[4], const uint32_t (&bh)[2], const float (&b)[2]) {

@@ -36,6 +36,12 @@ void check_float(const char* op, const char* name, const Tensor& t) {
 // The last check: what came before it needs no GPU.
 void check_gpu(const char* op, const Tensor& t) { TORCH_CHECK(t.is_cuda(), op, ": the input is on ", t.device(), ", not on a GPU"); }
 
+bool capturing(const Tensor& t) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream(t.get_device()).stream(), &status) == cudaSuccess &&
+         status != cudaStreamCaptureStatusNone;
+}
+
 // A gradient that goes to `t` ends in the node that adds it to t.grad, on the stream that node was made on.  In a capture that has
 // to be the capturing stream: a node left by an eager graph that is still alive is on another one, and the engine's waiting for it
 // would break the capture off from inside the backward pass.
@@ -43,9 +49,8 @@ void check_capture(const char* op, std::initializer_list<const Tensor*> tensors)
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : tensors) {
     if (!t->defined() || !t->is_leaf() || !t->requires_grad()) continue;
+    if (!capturing(*t)) return;
     const auto stream = c10::cuda::getCurrentCUDAStream(t->get_device());
-    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(stream.stream(), &status) != cudaSuccess || status == cudaStreamCaptureStatusNone) return;
     const auto* meta = torch::autograd::impl::get_autograd_meta(*t);
     const auto node = meta != nullptr ? meta->grad_accumulator_.lock() : nullptr;
     if (!node) continue;

@@ -5,6 +5,10 @@
     python -m eagersgd_b200.ops.bench_ops --op conv_wgrad --shape 64,128,28,28,128,3,1
     python -m eagersgd_b200.ops.bench_ops --op bn --shape 256,256,56,56 [--backward]
     python -m eagersgd_b200.ops.bench_ops --op lstm --shape 64,16,2048,2048              (T,B,I,H)
+    python -m eagersgd_b200.ops.bench_ops --op group_norm --shape 128,256,56,56,32       (N,C,H,W,groups) [--backward] [--residual]
+    python -m eagersgd_b200.ops.bench_ops --op causal_conv --shape 16,331,2048,4         (B,T,D,K) [--backward]
+    python -m eagersgd_b200.ops.bench_ops --op scan --shape 16,331,2048,16               (B,T,D,N) [--backward]
+    python -m eagersgd_b200.ops.bench_ops --op distill --shape 4096,32000,64             (rows,classes,top)
     python -m eagersgd_b200.ops.bench_ops --op suite
 
 Timing: 3 warm-up calls, then ``--iters`` calls between CUDA events on the launching stream with a
@@ -180,6 +184,88 @@ def bench_ce(shape, iters):
     return dict(op="softmax_ce_fwd+grad", B=b, C=c, ms=ms, gbs=3 * b * c * 4.0 / ms / 1e6, library_ms=ms_lib)
 
 
+def _grad_times(fn, lib, leaves, g, iters):
+    """ms of the backward pass alone, of the kernels and of the PyTorch restatement."""
+    from . import functional as ops
+    y = fn()
+    ms = timeit(lambda: torch.autograd.grad(y, leaves, g, retain_graph=True), iters)
+    with ops.reference_ops():
+        y2 = lib()
+        ms_lib = timeit(lambda: torch.autograd.grad(y2, leaves, g, retain_graph=True), max(1, iters // 3), graph=False)
+    return ms, ms_lib
+
+
+def bench_group_norm(shape, iters, backward=False, residual=False):
+    from . import functional as ops
+    n, c, h, w, groups = shape
+    x = _cl(torch.randn(n, c, h, w, device="cuda")).to(torch.bfloat16).requires_grad_()
+    res = _cl(torch.randn(n, c, h, w, device="cuda")).to(torch.bfloat16).requires_grad_() if residual else None
+    gamma, beta = torch.ones(c, device="cuda", requires_grad=True), torch.zeros(c, device="cuda", requires_grad=True)
+    fn = lambda: ops.group_norm_act(x, groups, gamma, beta, "silu", res)
+    if backward:
+        leaves = (x, gamma, beta) + ((res,) if residual else ())
+        ms, ms_lib = _grad_times(fn, fn, leaves, _cl(torch.randn_like(x)), iters)
+        byts = 2.0 * x.numel() * (5 if residual else 3)
+    else:
+        with torch.no_grad():
+            ms = timeit(fn, iters)
+            with ops.reference_ops():
+                ms_lib = timeit(fn, iters)
+        byts = 2.0 * x.numel() * (3 if residual else 2)
+    return dict(op="group_norm_silu_bwd" if backward else "group_norm_silu_fwd", N=n, C=c, H=h, W=w, groups=groups, residual=residual, ms=ms,
+                gbs=byts / ms / 1e6, library_ms=ms_lib)
+
+
+def bench_causal_conv(shape, iters, backward=False):
+    from . import functional as ops
+    from .scan import causal_conv
+    b, t, d, k = shape
+    x = torch.randn(b, t, d, device="cuda").to(torch.bfloat16).requires_grad_()
+    w, bias = torch.randn(d, k, device="cuda", requires_grad=True), torch.zeros(d, device="cuda", requires_grad=True)
+    fn = lambda: causal_conv(x, w, bias)
+    if backward:
+        ms, ms_lib = _grad_times(fn, fn, (x, w, bias), torch.randn_like(x), iters)
+    else:
+        with torch.no_grad():
+            ms = timeit(fn, iters)
+            with ops.reference_ops():
+                ms_lib = timeit(fn, iters)
+    return dict(op="causal_conv_bwd" if backward else "causal_conv_fwd", B=b, T=t, D=d, K=k, ms=ms,
+                gbs=2.0 * x.numel() * (3 if backward else 2) / ms / 1e6, library_ms=ms_lib)
+
+
+def bench_scan(shape, iters, backward=False):
+    from . import functional as ops
+    from .scan import selective_scan
+    b, t, d, n = shape
+    seq = lambda last: torch.randn(b, t, last, device="cuda").to(torch.bfloat16).requires_grad_()
+    u, delta, z, B, C = seq(d), seq(d), seq(d), seq(n), seq(n)
+    A = (-torch.arange(1, n + 1, device="cuda").float().repeat(d, 1)).requires_grad_()
+    D, bias = torch.ones(d, device="cuda", requires_grad=True), torch.full((d,), -4.0, device="cuda", requires_grad=True)
+    fn = lambda: selective_scan(u, delta, A, B, C, D, z, bias)
+    if backward:
+        ms, ms_lib = _grad_times(fn, fn, (u, delta, A, B, C, D, z, bias), torch.randn_like(u), iters)
+    else:
+        with torch.no_grad():
+            ms = timeit(fn, iters)
+            with ops.reference_ops():
+                ms_lib = timeit(fn, max(1, iters // 3), graph=False)
+    byts = 2.0 * u.numel() * (7 if backward else 4) + 4.0 * B.numel() * (2 if backward else 1)
+    return dict(op="selective_scan_bwd" if backward else "selective_scan_fwd", B=b, T=t, D=d, N=n, ms=ms, gbs=byts / ms / 1e6, library_ms=ms_lib)
+
+
+def bench_distill(shape, iters):
+    from . import functional as ops
+    rows, classes, top = shape
+    logits = torch.randn(rows, classes, device="cuda").to(torch.bfloat16).requires_grad_()
+    values, named = torch.randn(rows, classes, device="cuda").topk(top)
+    fn = lambda: ops.distillation_loss(logits, values, named, 2.0)
+    ms = timeit(fn, iters)
+    with ops.reference_ops():
+        ms_lib = timeit(lambda: torch.autograd.grad(fn(), logits), iters, graph=False)
+    return dict(op="distill_fwd+grad", rows=rows, classes=classes, top=top, ms=ms, gbs=4.0 * rows * classes / ms / 1e6, library_ms=ms_lib)
+
+
 def bench_lstm(shape, iters):
     """One LSTM layer, forward + backward: T steps of batch B, input I, hidden H (one persistent kernel per direction where the
     shape allows it) against torch.nn.LSTM (cuDNN)."""
@@ -266,6 +352,14 @@ def run(op, shape, iters, backward=False, residual=False):
         r = bench_ce(shape, iters)
     elif op == "lstm":
         r = bench_lstm(shape, iters)
+    elif op == "group_norm":
+        r = bench_group_norm(shape, iters, backward, residual)
+    elif op == "causal_conv":
+        r = bench_causal_conv(shape, iters, backward)
+    elif op == "scan":
+        r = bench_scan(shape, iters, backward)
+    elif op == "distill":
+        r = bench_distill(shape, iters)
     elif op == "update":
         r = bench_update(shape, iters)
     elif op == "lars":

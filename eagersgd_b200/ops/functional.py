@@ -258,7 +258,7 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     log_p = torch.log_softmax(torch.where(taught, values, 0.0), 1)
     log_q = torch.log_softmax(wide / t, 1).gather(1, teacher_classes.clamp(0, classes - 1))
     p = torch.where(named, log_p.exp(), 0.0)
-    kl = torch.where(p > 0, p * (torch.where(p > 0, log_p, 0.0) - torch.where(p > 0, log_q, 0.0)), 0.0).sum(1)
+    kl = torch.where(p != 0, p * (torch.where(p != 0, log_p, 0.0) - torch.where(p != 0, log_q, 0.0)), 0.0).sum(1)
     loss = (1.0 - hard_weight) * t * t * kl.sum() / logits.shape[0]
     if hard_weight != 0:
         valid = (labels >= 0) & (labels < classes)

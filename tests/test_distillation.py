@@ -194,6 +194,60 @@ def test_captured_with_its_backward_pass():
 
 
 @gpu
+def test_a_teacher_of_nan():
+    """No row without a teacher: the loss and the row's gradient are NaN, on the GPU as in the formula, and the other rows' are not."""
+    for top in (1, 5):
+        logits, values, named, _ = _case(3, 40, top, F32)
+        values[1] = float("nan")
+        for leaf, v, n in ((logits, values, named), (logits.cpu(), values.cpu(), named.cpu())):
+            leaf = leaf.detach().requires_grad_()
+            loss = ops.distillation_loss(leaf, v, n)
+            grad, = torch.autograd.grad(loss, leaf)
+            assert torch.isnan(loss) and torch.isnan(grad[1, n[1]]).all() and torch.isfinite(grad[[0, 2]]).all()
+
+
+@gpu
+def test_a_captured_backward_pass_alone():
+    """A forward pass made once, its backward pass captured: every replay gives the same gradient."""
+    logits, values, named, _ = _case(5, 77, 6, BF16)
+    factor = torch.tensor(0.5, device="cuda")
+    leaf = logits.requires_grad_()
+    want, = torch.autograd.grad(ops.distillation_loss(leaf, values, named), leaf, factor)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        loss = ops.distillation_loss(leaf, values, named)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got, = torch.autograd.grad(loss, leaf, factor)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@gpu
+def test_logits_past_32_bits():
+    """More than 2^31 of them: the last rows' loss and gradient are those of the rows alone."""
+    rows, classes = 70003, 32008
+    logits = torch.empty(rows, classes, dtype=BF16, device="cuda")
+    logits[:-2] = 0
+    small, values, named, _ = _case(2, classes, 5, BF16)
+    logits[-2:] = small
+    all_values, all_named = torch.zeros(rows, 5, device="cuda"), torch.full((rows, 5), -1, dtype=torch.int64, device="cuda")
+    all_values[-2:], all_named[-2:] = values.float(), named
+    leaf = logits.requires_grad_()
+    loss = ops.distillation_loss(leaf, all_values, all_named)
+    grad, = torch.autograd.grad(loss, leaf, torch.tensor(float(rows), device="cuda"))
+    ref = small.requires_grad_()
+    want = ops.distillation_loss(ref, values.float(), named)
+    want_grad, = torch.autograd.grad(want, ref, torch.tensor(2.0, device="cuda"))
+    assert abs(loss.item() * rows - want.item() * 2) < 1e-4 * want.item()
+    # both are rounded to bf16, times their row's weight, and again, times the factor; a named class is a difference of fp32 fractions
+    assert ((grad[-2:].float() - want_grad.float()).abs() <= 4.1 * 2.0 ** -8 * want_grad.float().abs() + 1e-6).all() and not grad[:-2].any()
+
+
+@gpu
 def test_gradient_against_differences():
     logits, values, named, labels = _case(2, 20, 4, F32)
     leaf = logits.detach().requires_grad_()

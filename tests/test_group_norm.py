@@ -187,6 +187,24 @@ def test_captured_on_its_own_stream_and_replayed():
 
 
 @gpu
+def test_images_past_32_bits():
+    x = torch.zeros(1100, 256, 128, 64, dtype=BF16, device="cuda").permute(0, 3, 1, 2)         # 2.3e9 values, channels last
+    g = torch.Generator().manual_seed(1)
+    x[-1:].copy_(_image(g, 1, 64, 256, 128))
+    gamma, beta = torch.randn(64, generator=g).cuda(), torch.randn(64, generator=g).cuda()
+    z = ops.group_norm_act(x, 4, gamma, beta, "silu")
+    want = ops.group_norm_act(x[-1:], 4, gamma, beta, "silu").double().cpu()
+    near(z[-1:], want, want.abs().max().item(), 4096, "z", roundings=2)      # split otherwise: sums in another order
+    del z
+    leaf = x.requires_grad_()
+    z = ops.group_norm_act(leaf, 4, gamma, beta, "silu")
+    dx, = torch.autograd.grad(z, leaf, x.detach())
+    one = x[-1:].detach().requires_grad_()
+    want, = torch.autograd.grad(ops.group_norm_act(one, 4, gamma, beta, "silu"), one, one.detach())
+    near(dx[-1:], want.double().cpu(), want.double().abs().max().item(), 4096, "dx", roundings=2)
+
+
+@gpu
 def test_gradient_against_differences():
     g = torch.Generator().manual_seed(10)
     x, dz, res = (_image(g, 1, 8, 3, 3, dtype=F32) for _ in range(3))

@@ -408,6 +408,66 @@ def test_empty_sequences_and_batches():
             assert g.shape == v.shape and not g.any()
 
 
+@gpu
+def test_rows_further_apart_than_32_bits():
+    """Slices of sequences whose rows and whose batch entries lie gigabytes apart."""
+    big = torch.empty(2, 3, 1 << 30, dtype=BF16, device="cuda")                # 12 GB: strides of 2^30 and 3 * 2^30
+    c, dy, _ = _scan_case(2, 3, 64, 16, BF16)
+    far = dict(c)
+    for i, k in enumerate(("u", "delta", "z", "B", "C")):
+        far[k] = big[:, :, (1 << 29) + 128 * i:(1 << 29) + 128 * i + c[k].shape[2]].copy_(c[k])
+    w, bias = torch.randn(64, 4, device="cuda"), torch.randn(64, device="cuda")
+    for f, names in ((lambda v: scan.selective_scan(**v), ("u", "delta", "z", "B", "C")), (lambda v: scan.causal_conv(v["u"], w, bias), ("u",))):
+        grads = []
+        for v in (c, far):
+            v = {k: t.detach().requires_grad_(k in names) for k, t in v.items()}
+            y = f(v)
+            grads.append((y.detach(), *torch.autograd.grad(y, [v[k] for k in names], dy)))
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+@gpu
+def test_expanded_operands():
+    """One sequence's steps for all, one step's operands for every step, and a gradient that is one number."""
+    c, _, _ = _scan_case(3, 11, 40, 16, F32)
+    shared = dict(c, B=c["B"][:1].expand(3, -1, -1), C=c["C"][:, :1].expand(-1, 11, -1), delta=c["delta"][:1, :1, :1].expand(3, 11, 40))
+    dense = {k: v.contiguous() for k, v in shared.items()}
+    got, want = ([], [])
+    for v, out in ((shared, got), (dense, want)):
+        leaves = {k: t.detach().requires_grad_() for k, t in v.items()}
+        y = scan.selective_scan(**leaves)
+        out += [y.detach(), *torch.autograd.grad(y.sum(), list(leaves.values()))]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_steps_in_inference_mode():
+    c, _, state = _scan_case(2, 3, 24, 16, BF16)
+    x, w, bias, _ = _conv_case(2, 5, 24, 4, BF16)
+    with torch.inference_mode():
+        last = torch.zeros(2, 3, 24, dtype=BF16, device="cuda")
+        ys = [scan.causal_conv_step(x[:, t], last, w, bias, out=last)[0] for t in range(5)]
+        h = state.clone()
+        for t in range(3):
+            now = {k: v if k in ("A", "D", "delta_bias") else v[:, t] for k, v in c.items()}
+            y, h = scan.selective_scan_step(**now, state=h, out=h)
+        want, want_h = scan.selective_scan(**c, state=state, return_state=True)
+    assert torch.equal(torch.stack(ys, 1), scan.causal_conv(x, w, bias))
+    assert torch.allclose(y.float(), want[:, 2].float(), rtol=2.0 ** -7, atol=1e-3) and torch.allclose(h, want_h, rtol=1e-5, atol=1e-5)
+
+
+@gpu
+def test_many_sequences_of_many_lengths():
+    """More sequences than a block has threads, and fewer: the order in which they are worked on is nobody's business."""
+    for b in (100, 200):
+        c, dy, _ = _scan_case(b, 24, 16, 4, F32)
+        lengths = torch.randint(0, 25, (b,), generator=_gen(b)).cuda()
+        got = scan.selective_scan(**c, lengths=lengths)
+        for i in (0, 1, b // 2, b - 1):
+            one = {k: v if k in ("A", "D", "delta_bias") else v[i:i + 1] for k, v in c.items()}
+            assert torch.equal(scan.selective_scan(**one, lengths=lengths[i:i + 1])[0], got[i])
+
+
 # ------------------------------------------------------------------------------------------------ without a GPU
 @pytest.mark.parametrize("dtype", [F32, torch.float64])
 def test_the_restatements_are_the_formulas(dtype):
