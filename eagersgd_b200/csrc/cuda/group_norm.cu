@@ -11,8 +11,13 @@
 // passes that follow; what does not fit there, and the residual, is read again and found in L2, of which what the resident
 // clusters work on at a time is a fraction.
 //
-// A CTA's variance is that about the CTA's own mean of each channel, and CTAs and channels are joined as means and squared
-// deviations: with sum and sum of squares a mean of 100 deviations would cost four digits.
+// Variances are squared deviations about a thread's, then a CTA's own mean of each channel, joined with the means: with sum and sum of
+// squares a mean of 100 deviations would cost four digits.
+//
+// 128 x 256 x 56 x 56 bf16, SiLU and residual: 160 us forward (3.9 TB/s of 6.5), 286 us backward (3.6 TB/s); 64 x 512 x 14 x 14: 11.5 and
+// 19 us.  The CTAs of a cluster wait for their slowest, and rows beyond the shared memory come out of L2 again.  Rows loaded at a time
+// by a thread, forward statistics 4 or 2: 32 x 64 x 112 x 112 47 or 51 us; backward 4, 2 or 6: 286, 307 or 368 us, and where all rows
+// are held 19.0, 18.2 or 19.2; forward results 2 or 4: 160 or 171 us (registers).
 #include <cooperative_groups.h>
 #include "launch.cuh"
 #include "rows.cuh"
@@ -136,6 +141,10 @@ template <class T, int kV, int kMany> struct Rows {
         }
     }
   }
+  // The vector of a thread's first row.
+  __device__ __forceinline__ Pack<T, kV> first(const Place<kV>& pl, int v) const {
+    return load<T, kV>(kV > 1 && pl.lane < held ? in + pl.lane * slice + v * kV : p[0] + pl.lane * pitch + v * kV);
+  }
   // use(vectors, the vector of `more`, their offset from p[]) for a thread's rows; kAhead of them are loaded at a time.
   template <int kAhead, bool kMore, class Use> __device__ __forceinline__ void each(const Place<kV>& pl, int v, const T* more, Use use) const {
     const int lanes = pl.lanes, n = kV == 1 ? 0 : held < pl.rows ? held : pl.rows, next = lanes * slice;
@@ -217,34 +226,47 @@ group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T
   in.ask(p);
   arrived();
   const float inv_rows = rows > 0 ? 1.0f / (float)rows : 0.0f;
+  // a thread's rows about its first one of a channel, which is one of them: what the squares lose to it is as many roundings as it
+  // has rows at most; threads, channels and CTAs are then joined as means and squared deviations
+  const float own_rows = (float)(rows > p.lane ? (rows - p.lane + p.lanes - 1) / p.lanes : 0), inv_own = own_rows > 0.0f ? 1.0f / own_rows : 0.0f;
   for (int v0 = 0; v0 < p.vectors; v0 += p.wide) {
     const int v = v0 + p.vec;
-    f2 a[1][kP] = {};
-    if (p.on(v))
-      in.template each<2, false>(p, v, nullptr, [&](const Pack<T, kV>(&raw)[1], const Pack<T, kV>&, int64_t) {
-        f2 f[kP];
-        unpack2<T, kV>(raw[0], f);
+    f2 a[1][kP] = {}, square[kP] = {}, first[kP] = {};
+    if (p.on(v) && p.lane < rows) {
+      unpack2<T, kV>(in.first(p, v), first);
 #pragma unroll
-        for (int q = 0; q < kP; ++q) a[0][q] = add2(a[0][q], f[q]);
-      });
-    channel_sums<1, kV>(p, a, v0, stage, mean, s.slice);
-  }
-  for (int v0 = 0; v0 < p.vectors; v0 += p.wide) {
-    const int v = v0 + p.vec;
-    f2 a[1][kP] = {}, m[kP];
-    if (p.on(v)) {
-      channels_of<kV>(mean + v * kV, m);
-#pragma unroll
-      for (int q = 0; q < kP; ++q) m[q] = mul2(m[q], -inv_rows);
-      in.template each<2, false>(p, v, nullptr, [&](const Pack<T, kV>(&raw)[1], const Pack<T, kV>&, int64_t) {
+      for (int q = 0; q < kP; ++q) first[q] = mul2(first[q], -1.0f);
+      in.template each<4, false>(p, v, nullptr, [&](const Pack<T, kV>(&raw)[1], const Pack<T, kV>&, int64_t) {
         f2 f[kP];
         unpack2<T, kV>(raw[0], f);
 #pragma unroll
         for (int q = 0; q < kP; ++q) {
-          const f2 d = add2(f[q], m[q]);
-          a[0][q] = fma2(d, d, a[0][q]);
+          const f2 d = add2(f[q], first[q]);
+          a[0][q] = add2(a[0][q], d);
+          square[q] = fma2(d, d, square[q]);
         }
       });
+    }
+    // from here: the thread's mean about -first, its squares about the mean, and its sum
+    f2 off[kP];
+#pragma unroll
+    for (int q = 0; q < kP; ++q) {
+      off[q] = mul2(a[0][q], inv_own);
+      square[q] = fma2(mul2(a[0][q], -1.0f), off[q], square[q]);
+      a[0][q] = fma2(first[q], -own_rows, a[0][q]);
+    }
+    channel_sums<1, kV>(p, a, v0, stage, mean, s.slice);
+    if (p.on(v)) {
+      f2 m[kP];
+      channels_of<kV>(mean + v * kV, m);
+#pragma unroll
+      for (int q = 0; q < kP; ++q) {
+        const f2 d = add2(off[q], mul2(add2(first[q], mul2(m[q], inv_rows)), -1.0f));
+        a[0][q] = fma2(mul2(d, own_rows), d, square[q]);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < kP; ++q) a[0][q] = 0;
     }
     channel_sums<1, kV>(p, a, v0, stage, m2, s.slice);
   }
@@ -379,7 +401,7 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
     f2 a[2][kP] = {};
     if (p.on(v)) {
       if (v0 > 0) coefficients(v);
-      in.template each<2, kRead>(p, v, residual + unit.base, [&](const Pack<T, kV>(&raw)[2], const Pack<T, kV>& more, int64_t) {
+      in.template each<4, kRead>(p, v, residual + unit.base, [&](const Pack<T, kV>(&raw)[2], const Pack<T, kV>& more, int64_t) {
         f2 f[kP], d[kP];
         derive(raw, more, f, d);
 #pragma unroll
@@ -441,7 +463,7 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
     channels_of<kV>(last + v * kV, kr);
     channels_of<kV>(last + s.slice + v * kV, a1);
     channels_of<kV>(last + 2 * s.slice + v * kV, a2);
-    in.template each<2, kRead>(p, v, residual + unit.base, [&](const Pack<T, kV>(&raw)[2], const Pack<T, kV>& more, int64_t o) {
+    in.template each<4, kRead>(p, v, residual + unit.base, [&](const Pack<T, kV>(&raw)[2], const Pack<T, kV>& more, int64_t o) {
       f2 f[kP], d[kP];
       derive(raw, more, f, d);
 #pragma unroll
@@ -456,7 +478,7 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
 // A slice has whole groups and whole vectors, and 128 bytes or more of a row where it can, so that a warp reads whole lines; more where
 // a slice of so few pixels is hardly worth a CTA, as long as all SMs have some (256x512x7x7: 27 -> 17 us forward).  A cluster has as
 // many CTAs as give three to every two SMs, and up to four so that its rows stay in shared memory, `budget` bytes a CTA for
-// `tensors` of them: 128x256x56x56 with residual forward / backward 180 / 321 us with two, 161 / 308 with four, 181 / 320 with eight.
+// `tensors` of them: 128x256x56x56 with residual forward / backward 180 / 321 us with two, 161 / 308 with four, 181 / 320 with eight (two rows at a time).
 // False where a slice is too wide.
 constexpr int kSmallUnit = 16 * 1024;
 bool plan(int64_t samples, int64_t rows, int channels, int groups, int v, int size, int tensors, int budget, Shape* s) {
