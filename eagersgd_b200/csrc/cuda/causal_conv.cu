@@ -5,7 +5,10 @@
 //
 // Bound by memory.  A thread has four channels and a run of steps, the window in registers: of every run only the K - 1 inputs ahead
 // of it are read twice (the backward pass makes the K - 1 dpre behind it again).  Eight channels a thread took twice the registers,
-// and half the warps were not enough loads in flight.
+// and half the warps were not enough loads in flight; two channels a thread, backward, took 263 us for 235: its instructions count.
+//
+// 64 x 1000 steps of 2048 channels, four taps, bf16: forward 112 us (4.7 TB/s of 6.5), backward 235 us (3.3); 16 x 331 steps, which L2
+// holds: 13.7 and 26 us.
 #include "launch.cuh"
 #include "rows.cuh"
 
@@ -14,7 +17,9 @@ namespace {
 using namespace esgd;
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;            // steps that are loaded at a time
+// steps that are loaded at a time, while those ahead of them are at work; backward 4 do not fit into the registers (261 -> 235 us with 2;
+// 1: 310 us, though 26 -> 23 us where all comes out of L2)
+constexpr int kAhead = 4, kBack = 2;
 
 struct Conv {
   int64_t batch, length;
@@ -125,12 +130,19 @@ __global__ void __launch_bounds__(kThreads) causal_conv_fwd_kernel(const T* __re
     f2 win[kTaps][kP];
 #pragma unroll
     for (int k = 0; k < kTaps - 1; ++k) input<T, kV>(x, state, p, s.b, s.first - (kTaps - 1) + k, s.c, kTaps, win[k + 1]);
+    Pack<T, kV> next[kAhead];
+    auto fetch = [&](int n) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (u < n) next[u] = load<T, kV>(in + u * p.xt);
+      in += kAhead * p.xt;
+    };
+    fetch(live);
     for (int t = 0; t < live; t += kAhead) {
       Pack<T, kV> raw[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (t + u < live) raw[u] = load<T, kV>(in + u * p.xt);
-      in += kAhead * p.xt;
+      for (int u = 0; u < kAhead; ++u) raw[u] = next[u];
+      fetch(live - t - kAhead);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         if (t + u >= live) break;
@@ -182,18 +194,28 @@ __global__ void __launch_bounds__(kThreads, 2) causal_conv_bwd_kernel(const T* _
         for (int k = 0; k < kTaps; ++k) win[k][q] = dp[k][q] = 0;
 #pragma unroll
       for (int k = 0; k < kTaps - 1; ++k) input<T, kV>(x, state, p, s.b, s.first - (kTaps - 1) + k, s.c, kTaps, win[k + 1]);
-      for (; t < steps + kTaps - 1; t += kAhead) {
-        Pack<T, kV> rx[kAhead], rd[kAhead];
+      Pack<T, kV> next_x[kBack], next_d[kBack];
+      auto fetch = [&](int n) {
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-          if (t + u < ahead) {
-            rx[u] = load<T, kV>(in + u * p.xt);
-            rd[u] = load<T, kV>(up + (int64_t)u * p.channels);
+        for (int u = 0; u < kBack; ++u)
+          if (u < n) {
+            next_x[u] = load<T, kV>(in + u * p.xt);
+            next_d[u] = load<T, kV>(up + (int64_t)u * p.channels);
           }
-        in += kAhead * p.xt;
-        up += (int64_t)kAhead * p.channels;
+        in += kBack * p.xt;
+        up += (int64_t)kBack * p.channels;
+      };
+      fetch(ahead);
+      for (; t < steps + kTaps - 1; t += kBack) {
+        Pack<T, kV> rx[kBack], rd[kBack];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
+        for (int u = 0; u < kBack; ++u) {
+          rx[u] = next_x[u];
+          rd[u] = next_d[u];
+        }
+        fetch(ahead - t - kBack);
+#pragma unroll
+        for (int u = 0; u < kBack; ++u) {
           if (t + u >= steps + kTaps - 1) break;
 #pragma unroll
           for (int q = 0; q < kP; ++q)
@@ -228,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 2) causal_conv_bwd_kernel(const T* _
             store2<T, kV>(out + (int64_t)u * p.channels, f);
           }
         }
-        out += (int64_t)kAhead * p.channels;
+        out += (int64_t)kBack * p.channels;
       }
     } else if (dx != nullptr) {
       const f2 zero[kP] = {};
@@ -274,16 +296,26 @@ __global__ void __launch_bounds__(128) causal_conv_step_kernel(const T* __restri
   for (int k = 0; k < kTaps - 1; ++k) store2<T, kV>(state_out + (b * (kTaps - 1) + k) * channels + c, win[k + 1]);
 }
 
-void plan(Conv* p, int v) {
+// Blocks of an SM at a time.
+constexpr int kForwardFull = 4, kBackwardFull = 2;
+void plan(Conv* p, int v, int full) {
   const int vectors = p->channels / v;
   p->lanes = 1;
   while (p->lanes < 32 && p->lanes < vectors) p->lanes *= 2;
   p->runs = kThreads / p->lanes;
   p->vec_blocks = (vectors + p->lanes - 1) / p->lanes;
-  // long runs read least twice; short ones fill the GPU
+  // The number of steps that is estimated to take least: a run begins with what takes as long as 12 steps, an SM has `full` blocks at a
+  // time, and a wave of few blocks takes as long as a full one (16 x 331 steps of 2048 channels, backward: 16 steps and three waves
+  // 33 us, 44 steps and one wave 26 us).
   p->steps = 64;
-  while (p->steps > 4 && p->batch * p->vec_blocks * ((p->length + (int64_t)p->runs * p->steps - 1) / (p->runs * p->steps)) < 4 * sm_count())
-    p->steps /= 2;
+  int64_t best = -1;
+  for (int steps = 64; steps >= 4; steps -= 4) {
+    const int64_t blocks = p->batch * p->vec_blocks * ((p->length + (int64_t)p->runs * steps - 1) / (p->runs * steps));
+    const int64_t cost = (blocks + full * sm_count() - 1) / (full * sm_count()) * (steps + 12);
+    if (best >= 0 && cost >= best) continue;
+    best = cost;
+    p->steps = steps;
+  }
   p->time_blocks = (int)((p->length + (int64_t)p->runs * p->steps - 1) / (p->runs * p->steps));
   if (p->time_blocks < 1) p->time_blocks = 1;
 }
@@ -336,7 +368,7 @@ int esgd_causal_conv_fwd(const void* x, int64_t xb, int64_t xt, const void* stat
   if (batch == 0 || channels == 0) return 0;
   const int v = width(is_bf16, channels, xb, xt, x, state, y, state_out);
   Conv p = {batch, length, channels, xb, xt, lengths, weight, bias};
-  plan(&p, v);
+  plan(&p, v, kForwardFull);
   return ESGD_TYPE(forward, x, state, y, state_out, p, stream);
 }
 
@@ -347,7 +379,7 @@ int64_t esgd_causal_conv_parts(int64_t batch, int64_t length, int channels) {
   for (int v : {1, 4}) {
     if (channels % v) continue;
     Conv p = {batch, length, channels};
-    plan(&p, v);
+    plan(&p, v, kBackwardFull);
     if (p.batch * p.time_blocks > most) most = p.batch * p.time_blocks;
   }
   return most;
@@ -362,7 +394,7 @@ int esgd_causal_conv_bwd(const void* x, int64_t xb, int64_t xt, const void* stat
   if (batch == 0 || channels == 0 || length == 0) return 0;
   const int v = width(is_bf16, channels, xb, xt, x, state, dy, dx);
   Conv p = {batch, length, channels, xb, xt, lengths, weight, bias};
-  plan(&p, v);
+  plan(&p, v, kBackwardFull);
   *parts = p.batch * p.time_blocks;
   return ESGD_TYPE(backward, x, state, dy, dx, sums, p, stream);
 }
