@@ -11,15 +11,20 @@
 //
 // One exponential a state and step, against some 8 bytes a channel and step: bound by the special function units and the issue of
 // instructions, not by memory.  States stay in registers over the whole sequence, those of two neighbouring channels in a 64-bit
-// register for the paired fp32 instructions.  A tile of steps is prepared elementwise (a thread: two neighbouring channels of a step; their operands are fetched
-// a tile ahead), goes through shared memory to the threads that have the states, and comes back for the sums over the states and
-// the gates.
+// register for the paired fp32 instructions.  A tile of steps is prepared elementwise (a thread: two neighbouring channels of a
+// step; their operands are fetched a tile ahead), goes through shared memory to the threads that have the states, and comes back
+// for the sums over the states and the gates.
 //
 // Forward: two channels' states lie in kLanes threads, two by four in each: with one channel to a thread the reads of B and C out
-// of shared memory (32 bytes a thread and step) took longer than the exponentials.  Backward: a warp has eight channels and sixteen states, a
-// thread two by two of them as the tensor cores' m16n8k8 fragments want them: the sums over the channels that dB and dC are, eight
-// values a thread and step, are two matrix instructions instead of some forty shuffles and additions.  The states ahead of every
-// eighth step are kept by the forward pass, so that the backward pass needs one exponential a state and step as well.
+// of shared memory (32 bytes a thread and step) took longer than the exponentials.  Backward: a warp has eight channels and sixteen
+// states, a thread two by two of them as the tensor cores' m16n8k8 fragments want them: the sums over the channels that dB and dC
+// are, eight values a thread and step, are two matrix instructions instead of some forty shuffles and additions.  The states ahead
+// of every eighth step are kept by the forward pass, so that the backward pass needs one exponential a state and step as well.
+//
+// 64 x 331 steps of 2048 channels, 16 states, bf16: forward 279 us (694 M exponentials, 154 us at 16 a clock and SM), backward 1024 us:
+// the partial sums' way through shared memory takes two thirds of its time there.  (The exponentials made again, instead of kept in
+// registers from the first half of a tile to the second, and four blocks an SM: 1061 us for 1035; arithmetic without pairs: 1125 for
+// 1072.)
 //
 // Few sequences of few channels: the steps are split into chunks that run at the same time.  A first pass scans every chunk from a
 // state of zero; what a chunk begins with is then the chunks ahead of it joined, h = exp(A sum dt) h + (its own scan).
@@ -345,6 +350,8 @@ __global__ void __launch_bounds__(kThreads) selective_scan_chunk_kernel(Scan s, 
   pdl_enter();
   using In = Lanes<kLanes>;
   constexpr int kWide = In::kWide, kPadded = In::kPadded;
+  // what leaves the last chunk goes nowhere
+  if ((int)(blockIdx.x / ((s.channels + kWide - 1) / kWide) % s.chunks) == (kReverse ? 0 : s.chunks - 1)) return;
   __shared__ float4 s_bc[kTile * kLanes];                  // B, or C
   __shared__ float4 s_dt[kTile * kWide / 2];               // of two channels: dt, and dt * u (or dy)
   const Block<kWide> p(s);
@@ -761,7 +768,8 @@ template <class T, bool kWhole> __device__ __forceinline__ void four(const T* p,
 }
 
 // One step of every sequence: the state moves on; state_out may be s.state.  A block has kWide channels of `many` sequences, one
-// after the other, each fetched while the one ahead is at work.  Bound by memory: 8 bytes a state.
+// after the other, each fetched while the one ahead is at work.  Bound by memory: 8 bytes a state (1000 sequences of 2048 channels with
+// 16 states: 65 us, 4.0 TB/s of 6.5; four states fetched at once 71 us, without softplus and gate it would be 61).
 template <class T, int kLanes, bool kWhole>
 __global__ void __launch_bounds__(kThreads) selective_scan_step_kernel(Scan s, float* state_out, T* __restrict__ out, int many) {
   pdl_enter();
@@ -829,13 +837,14 @@ int blocks_of(int channels, int wide) { return (channels + wide - 1) / wide; }
 
 // Chunks of a pass over `blocks` blocks, the number that is estimated to take least.  A block takes as long as its steps, a start of
 // some 24 steps, and the chunks ahead of it to join; an SM has `full` blocks at the pace of one, and takes longer with more, up to
-// `most` at a time; with chunks there is a pass more, and all that is done `again` times.  Forward, us without and with them:
-// 1 x 4099 steps of 2048 channels 930 / 129 (29 chunks), 2 x 500 of 4096 146 / 62, 8 x 120 of 2048 26 / 35.
+// `most` at a time; with chunks there is a pass more, and all that is done `again` times.  Us without and with them, forward and
+// backward: 1 x 4099 steps of 2048 channels 513 / 119 and 784 / 291, 1 x 2000 of 64 250 / 23 and 369 / 30, 4 x 1000 of 2048 128 / 102
+// and 329 / 265; 16 x 200 of 1024 would take 35 / 61 forward and has none.
 struct Pace {
   double full, again;
   int64_t most;
 };
-constexpr Pace kForward = {4.2, 1.9, 8}, kBackward = {3.0, 1.35, 3};
+constexpr Pace kForward = {4.2, 1.9, 8}, kBackward = {3.0, 1.25, 3};
 void split(Scan* s, int64_t blocks, const Pace& p) {
   double best = 0.0;
   for (int64_t n = 1; n <= kMaxChunks; n *= 2) {
