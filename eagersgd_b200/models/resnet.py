@@ -51,6 +51,13 @@ class BatchNormAct(nn.BatchNorm2d):
                           residual, stats, self.training)
 
 
+def _bn(ch: int, zero_gamma: bool = False) -> BatchNormAct:
+    bn = BatchNormAct(ch, eps=BN_EPS, momentum=1.0 - BN_MOMENTUM_TF)
+    if zero_gamma:
+        nn.init.zeros_(bn.weight)
+    return bn
+
+
 class GroupNormAct(nn.GroupNorm):
     """Group norm in the place of ``BatchNormAct``: no statistics of the batch, so replicas that see other samples, or miss a
     round, compute the same function, and a batch of one is as good as any."""
@@ -64,14 +71,13 @@ NORM_GROUPS = 32
 
 def _norm(norm: str, ch: int, zero_gamma: bool = False) -> nn.Module:
     """``group``: 32 groups at most, of eight channels or more."""
-    if norm == "group":
-        groups = max(g for g in range(1, NORM_GROUPS + 1) if ch % g == 0 and (ch // g >= 8 or g == 1))
-        m = GroupNormAct(groups, ch, eps=BN_EPS)
-    else:
-        m = BatchNormAct(ch, eps=BN_EPS, momentum=1.0 - BN_MOMENTUM_TF)
+    if norm == "batch":
+        return _bn(ch, zero_gamma)
+    groups = max(g for g in range(1, NORM_GROUPS + 1) if ch % g == 0 and (ch // g >= 8 or g == 1))
+    gn = GroupNormAct(groups, ch, eps=BN_EPS)
     if zero_gamma:
-        nn.init.zeros_(m.weight)
-    return m
+        nn.init.zeros_(gn.weight)
+    return gn
 
 
 class _Conv(nn.Conv2d):
@@ -81,9 +87,11 @@ class _Conv(nn.Conv2d):
     squares of ``y`` when the kernel produced them in its epilogue (else ``None``).
     """
 
+    statistics = True                        # whether a batch norm follows, which uses them (also of layers saved without it)
+
     def __init__(self, cin, cout, k, stride, statistics=True):
         super().__init__(cin, cout, k, stride=stride, padding=(k - 1) // 2, bias=False)
-        self.statistics = statistics         # whether a batch norm follows, which uses them
+        self.statistics = statistics
         # variance_scaling_initializer() of the reference: fan-in scaling
         nn.init.kaiming_normal_(self.weight, mode="fan_in", nonlinearity="linear")
 
@@ -184,6 +192,8 @@ class _Block(nn.Module):
 
 
 class ResNet(nn.Module):
+    norm = "batch"                           # also of networks that were saved without it
+
     def __init__(self, kind: str, blocks: List[int], num_classes: int, num_filters: int, first_kernel: int,
                  first_stride: int, first_pool: bool, block_strides: List[int], version: int = 1, norm: str = "batch"):
         super().__init__()
