@@ -14,7 +14,7 @@
 // Variances are squared deviations about a thread's, then a CTA's own mean of each channel, joined with the means: with sum and sum of
 // squares a mean of 100 deviations would cost four digits.
 //
-// 128 x 256 x 56 x 56 bf16, SiLU and residual: 160 us forward (3.9 TB/s of 6.5), 286 us backward (3.6 TB/s); 64 x 512 x 14 x 14: 11.5 and
+// 128 x 256 x 56 x 56 bf16, SiLU and residual: 160 us forward (3.9 TB/s of 6.5), 273 us backward (3.8 TB/s); 64 x 512 x 14 x 14: 11.5 and
 // 19 us.  The CTAs of a cluster wait for their slowest, and rows beyond the shared memory come out of L2 again.  Rows loaded at a time
 // by a thread, forward statistics 4 or 2: 32 x 64 x 112 x 112 47 or 51 us; backward 4, 2 or 6: 286, 307 or 368 us, and where all rows
 // are held 19.0, 18.2 or 19.2; forward results 2 or 4: 160 or 171 us (registers).
@@ -36,11 +36,32 @@ struct Shape {
   int slice;           // channels of a slice: whole groups
   int split;           // CTAs of a cluster
   int held;            // rows of a CTA that stay in shared memory
+  int passing;         // nothing of a tensor is in L2 when the next operator reads it
   float eps;
 };
 
 // The backward pass' sums of two sets, and later three rows of coefficients.
 __host__ __device__ constexpr int stage_floats(int v, int slice) { return 2 * kThreads * v > 3 * slice ? 2 * kThreads * v : (3 * slice + 3) / 4 * 4; }
+
+// How L2 keeps what the backward pass fetches once or writes: as ever, or, of tensors that it cannot hold, less long than the rows that
+// are fetched again (128 x 256 x 56 x 56 with residual: 286 -> 273 us; forward the registers for it cost more than it brings,
+// 32 x 64 x 112 x 112: 47 -> 51).
+__device__ __forceinline__ uint64_t l2_policy(const Shape& s) {
+  uint64_t first, normal;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
+  asm("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(normal));
+  return s.passing ? first : normal;
+}
+template <class T, int kV> __device__ __forceinline__ void leave2(T* p, const f2 (&f)[PairsOf<kV>::n], uint64_t policy) {
+  if constexpr (kV == 1) {
+    store2<T, kV>(p, f);
+  } else {
+    uint4 w;
+    store2<T, kV>(reinterpret_cast<T*>(&w), f);
+    asm volatile("st.global.L2::cache_hint.v4.b32 [%0], {%1, %2, %3, %4}, %5;" ::"l"(p), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w), "l"(policy)
+                 : "memory");
+  }
+}
 
 // Where a thread works: a vector of kV channels, every `lanes`-th row of its CTA's.
 template <int kV> struct Place {
@@ -125,7 +146,7 @@ template <class T, int kV, int kMany> struct Rows {
   int held, slice;
   int64_t pitch;
   __device__ Rows(T* in_, const Shape& s) : in(in_), held(s.held), slice(s.slice), pitch(s.channels) {}
-  __device__ __forceinline__ void ask(const Place<kV>& pl) const {
+  template <bool kPolicy> __device__ __forceinline__ void ask(const Place<kV>& pl, uint64_t policy = 0) const {
     if constexpr (kV > 1) {
       const int n = held < pl.rows ? held : pl.rows;
       for (int v = pl.vec; pl.on(v); v += pl.wide)
@@ -134,7 +155,10 @@ template <class T, int kV, int kMany> struct Rows {
           const T* from = p[i] + pl.lane * pitch + v * kV;
           uint32_t to = (uint32_t)__cvta_generic_to_shared(in + (i * held + pl.lane) * slice + v * kV);
           for (int r = pl.lane; r < n; r += pl.lanes) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+            if constexpr (kPolicy)
+              asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "l"(policy) : "memory");
+            else
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
             from += pl.lanes * pitch;
             to += pl.lanes * slice * (int)sizeof(T);
           }
@@ -223,7 +247,7 @@ group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T
   in.p[0] = x + unit.base;
   constexpr int kP = PairsOf<kV>::n;
   const int rows = p.rows;
-  in.ask(p);
+  in.ask<false>(p);
   arrived();
   const float inv_rows = rows > 0 ? 1.0f / (float)rows : 0.0f;
   // a thread's rows about its first one of a channel, which is one of them: what the squares lose to it is as many roundings as it
@@ -360,7 +384,8 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
   in.p[1] = dz + unit.base;
   constexpr int kP = PairsOf<kV>::n;
   constexpr bool kRead = kAdd && kAct != kActNone;         // the residual moves the activation's slope
-  in.ask(p);
+  const uint64_t policy = l2_policy(s);
+  in.ask<true>(p, policy);
   const float* st = stats + 2 * (unit.sample * (s.channels / s.per) + unit.c0 / s.per);
   for (int c = threadIdx.x; c < s.slice; c += kThreads) {
     const int g = c / s.per;
@@ -468,8 +493,8 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
       derive(raw, more, f, d);
 #pragma unroll
       for (int q = 0; q < kP; ++q) f[q] = fma2(f[q], a2[q], fma2(d[q], kr[q], a1[q]));
-      if (dx != nullptr) store2<T, kV>(dx + unit.base + o, f);
-      if (dres != nullptr) store2<T, kV>(dres + unit.base + o, d);
+      if (dx != nullptr) leave2<T, kV>(dx + unit.base + o, f, policy);
+      if (dres != nullptr) leave2<T, kV>(dres + unit.base + o, d, policy);
     });
   }
   if (s.split > 1) cluster.barrier_wait();        // nobody leaves while its sums are being read
@@ -481,6 +506,7 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
 // `tensors` of them: 128x256x56x56 with residual forward / backward 180 / 321 us with two, 161 / 308 with four, 181 / 320 with eight (two rows at a time).
 // False where a slice is too wide.
 constexpr int kSmallUnit = 16 * 1024;
+constexpr int64_t kPassing = 32 << 20;      // bytes; a backward pass has three to five such tensors, L2 room for four
 bool plan(int64_t samples, int64_t rows, int channels, int groups, int v, int size, int tensors, int budget, Shape* s) {
   s->rows = rows;
   s->channels = channels;
@@ -500,6 +526,7 @@ bool plan(int64_t samples, int64_t rows, int channels, int groups, int v, int si
     s->split *= 2;
   const int64_t held = v > 1 ? budget / row : 0, most = (rows + s->split - 1) / s->split;
   s->held = (int)(held < most ? held : most);
+  s->passing = samples * rows * channels * size > kPassing;
   return true;
 }
 
