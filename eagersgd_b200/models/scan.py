@@ -15,6 +15,7 @@ import torch.nn as nn
 
 from ..ops import functional as ops
 from ..ops import scan
+from .resnet import GroupNormAct
 
 State = List[Tuple[torch.Tensor, torch.Tensor]]
 
@@ -30,7 +31,7 @@ class ScanLayer(nn.Module):
         self.hidden, self.width, self.states = hidden, width, states
         self.rank = step_rank or max(8, (width // 16 + 7) // 8 * 8)
         uniform = lambda *s: nn.Parameter(torch.empty(*s).uniform_(-1, 1) / math.sqrt(s[-1]))  # noqa: E731
-        self.norm = nn.GroupNorm(1, hidden)
+        self.norm = GroupNormAct(1, hidden)
         self.w_in = uniform(2 * width, hidden)
         self.conv_weight, self.conv_bias = uniform(width, taps), nn.Parameter(torch.zeros(width))
         self.w_bc = uniform(self.rank + 2 * states, width)
@@ -49,7 +50,7 @@ class ScanLayer(nn.Module):
         return self
 
     def _ahead(self, h):
-        x = ops.group_norm_act(h.reshape(h.shape[0], self.hidden, 1, 1), 1, self.norm.weight, self.norm.bias, eps=self.norm.eps)
+        x = self.norm(h.reshape(h.shape[0], self.hidden, 1, 1), relu=False)
         return _project(x.reshape(h.shape), self.w_in)
 
     def _operands(self, u):
@@ -119,7 +120,7 @@ class ScanClassifier(nn.Module):
     def _last(self, h, lengths):
         if lengths is None:
             return h[:, -1]
-        return h[torch.arange(h.shape[0], device=h.device), lengths.clamp(min=1) - 1]
+        return h[torch.arange(h.shape[0], device=h.device), lengths.clamp(1, h.shape[1]) - 1]
 
     def forward(self, x, lengths=None):
         """x [B, T, input_dim] -> logits [B, classes] of every sequence's last step."""

@@ -128,6 +128,9 @@ def main(argv=None):
     p.add_argument("--synthetic_train_size", type=int, default=None, help="samples per epoch of synthetic data")
     p.set_defaults(resnet_size=None, train_epochs=None, epochs_between_evals=None)      # filled in per data set below
     args = F.resolve(p.parse_args(argv))
+    for flag in ("export_dir", "pretrained_model_checkpoint_path", "virtual_batch_size"):
+        if args.norm == "group" and getattr(args, flag):
+            p.error("--%s is about batch norm: not with --norm group" % flag)
     info = DATASETS[args.dataset]
     if args.resnet_size is None:
         args.resnet_size = info["default_size"]

@@ -21,6 +21,7 @@ import contextlib
 import torch
 import torch.nn as nn
 
+from ..models.resnet import GroupNormAct
 from ..optim.eager import MajorityAllreduceOptimizer, SoloAllreduceOptimizer, SyncAllreduceOptimizer
 from ..parallel import _native as N
 from ..parallel.group import Group
@@ -95,7 +96,8 @@ class TrainStep:
         """All parameters in one group, or — to keep weight decay off the normalisation layers — two."""
         if decay_norm_params or not weight_decay:
             return list(model.parameters())
-        norm = {id(p) for m in model.modules() if isinstance(m, (nn.modules.batchnorm._BatchNorm, nn.GroupNorm)) for p in m.parameters(recurse=False)}
+        norm = {id(p) for m in model.modules() if isinstance(m, (nn.modules.batchnorm._BatchNorm, GroupNormAct))
+                for p in m.parameters(recurse=False)}
         decayed = [p for p in model.parameters() if id(p) not in norm]
         plain = [p for p in model.parameters() if id(p) in norm]
         if not plain:

@@ -84,6 +84,30 @@ def test_decay_checkpoints_and_flags_know_group_norm():
     assert build_model(args, DATASETS["cifar10"]).norm == "group"
 
 
+@pytest.mark.parametrize("flag", ["--export_dir", "--pretrained_model_checkpoint_path", "--virtual_batch_size"])
+def test_what_is_about_batch_norm_is_refused_before_training(flag, capsys):
+    from eagersgd_b200.train import resnet_main
+    with pytest.raises(SystemExit):
+        resnet_main.main(["--norm", "group", "--dataset", "cifar10", flag, "4"])
+    assert "not with --norm group" in capsys.readouterr().err
+
+
+def test_lengths_beyond_the_sequence_end_with_it():
+    net = ScanClassifier(8, 16, 1, 5)
+    x = torch.randn(3, 6, 8)
+    want = net(x, torch.tensor([6, 6, 1]))
+    assert torch.equal(net(x, torch.tensor([9, 1 << 40, -2]))[:2], want[:2])
+    assert torch.isfinite(net(x, torch.tensor([9, 6, -2]))).all()
+
+
+def test_a_users_own_group_norm_decays_as_it_did():
+    from eagersgd_b200.train.step import TrainStep
+    own = torch.nn.Sequential(torch.nn.Conv2d(3, 8, 1), torch.nn.GroupNorm(2, 8), torch.nn.BatchNorm2d(8))
+    decayed, plain = TrainStep._param_groups(own, 1e-4, False)
+    assert {id(p) for p in plain["params"]} == {id(p) for p in own[2].parameters()}
+    assert any(p is own[1].weight for p in decayed["params"])
+
+
 def test_clips_through_a_scan():
     frames = torch.nn.Module()
     frames.features = lambda x: x.mean((2, 3)).repeat(1, 4)
