@@ -203,6 +203,7 @@ Tensor zeros_f32(at::IntArrayRef shape, at::Device device) {
 class GradSinks;
 struct SinkEntry : torch::CustomClassHolder {
   float* acc = nullptr;          // fp32 accumulator, in the parameter's own memory order (OHWI for channels_last filters)
+  c10::Storage room;             // ... and its memory, which has to last as long as an operator may write it
   int bucket = 0;
   c10::weak_intrusive_ptr<at::TensorImpl, at::UndefinedTensorImpl> param;
   // of the step that is under way:
@@ -253,6 +254,7 @@ class GradSinks {
     TORCH_CHECK(acc.scalar_type() == at::kFloat && acc.numel() == param.numel());
     auto e = c10::make_intrusive<SinkEntry>(param);
     e->acc = acc.data_ptr<float>();
+    e->room = acc.storage();
     e->bucket = bucket;
     e->owner.store(this);
     std::unique_lock<std::shared_mutex> g(g_sink_mutex);
