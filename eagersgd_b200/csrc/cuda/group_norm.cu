@@ -44,8 +44,8 @@ struct Shape {
 __host__ __device__ constexpr int stage_floats(int v, int slice) { return 2 * kThreads * v > 3 * slice ? 2 * kThreads * v : (3 * slice + 3) / 4 * 4; }
 
 // How L2 keeps what the backward pass fetches once or writes: as ever, or, of tensors that it cannot hold, less long than the rows that
-// are fetched again (128 x 256 x 56 x 56 with residual: 286 -> 273 us, 885 -> 744 MB read for 616; forward the registers for it cost more than it brings,
-// 32 x 64 x 112 x 112: 47 -> 51).
+// are fetched again (128 x 256 x 56 x 56 with residual: 286 -> 273 us, 885 -> 744 MB read for 616; forward the registers for it cost
+// more than it brings, 32 x 64 x 112 x 112: 47 -> 51 us).
 __device__ __forceinline__ uint64_t l2_policy(const Shape& s) {
   uint64_t first, normal;
   asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
@@ -503,7 +503,8 @@ group_norm_bwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, c
 // A slice has whole groups and whole vectors, and 128 bytes or more of a row where it can, so that a warp reads whole lines; more where
 // a slice of so few pixels is hardly worth a CTA, as long as all SMs have some (256x512x7x7: 27 -> 17 us forward).  A cluster has as
 // many CTAs as give three to every two SMs, and up to four so that its rows stay in shared memory, `budget` bytes a CTA for
-// `tensors` of them: 128x256x56x56 with residual forward / backward 180 / 321 us with two, 161 / 308 with four, 181 / 320 with eight (two rows at a time).
+// `tensors` of them: 128x256x56x56 with residual forward / backward, two rows loaded at a time, 180 / 321 us with two, 161 / 308 with
+// four, 181 / 320 with eight.
 // False where a slice is too wide.
 constexpr int kSmallUnit = 16 * 1024;
 constexpr int64_t kPassing = 32 << 20;      // bytes; a backward pass has three to five such tensors, L2 room for four
