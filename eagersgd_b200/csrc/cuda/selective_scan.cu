@@ -18,11 +18,11 @@
 // Forward: two channels' states lie in kLanes threads, two by four in each: with one channel to a thread the reads of B and C out
 // of shared memory (32 bytes a thread and step) took longer than the exponentials.  Backward: a warp has eight channels and sixteen
 // states, a thread two by two of them as the tensor cores' m16n8k8 fragments want them: the sums over the channels that dB and dC
-// are, eight values a thread and step, are two matrix instructions instead of some forty shuffles and additions.  The states ahead
+// are, eight values a thread and step, are four matrix instructions instead of some forty shuffles and additions.  The states ahead
 // of every eighth step are kept by the forward pass, so that the backward pass needs one exponential a state and step as well.
 //
-// 64 x 331 steps of 2048 channels, 16 states, bf16: forward 279 us (694 M exponentials, 154 us at 16 a clock and SM), backward 1024 us:
-// the partial sums' way through shared memory takes two thirds of its time there.  (The exponentials made again, instead of kept in
+// 64 x 331 steps of 2048 channels, 16 states, bf16: forward 279 us (694 M exponentials, 154 us at 16 a clock and SM), backward 1230 us:
+// the partial sums' way through shared memory takes half of its time there.  (The exponentials made again, instead of kept in
 // registers from the first half of a tile to the second, and four blocks an SM: 1061 us for 1035; arithmetic without pairs: 1125 for
 // 1072.)
 //
@@ -40,6 +40,7 @@ constexpr int kThreads = 128;
 constexpr int kStates = 4;           // of a thread and channel, forward
 constexpr int kTile = 16;            // steps of a tile, forward
 constexpr int kKeep = 8;             // steps between kept states, and of a tile of the backward pass
+constexpr int kHalf = kKeep / 2;     // steps that a matrix product's columns hold
 constexpr int kMaxChunks = 64;
 
 // [batch][length][width]: strides in elements, the last one is 1.
@@ -460,31 +461,29 @@ struct Grads {
   float* sums;                 // [batch][chunks][channels * states + channels + channels]: dA, dD, ddelta_bias
 };
 
-// The matrix instruction reads eleven bits of a factor: half a step of these more, and leaving the others out rounds to the nearest.
-__device__ __forceinline__ uint32_t tf32(float x) { return __float_as_uint(x) + 0x1000u; }
+// The matrix instruction reads the upper eleven bits of a factor and leaves out the others: what that is, and (fp32 gradients) half a step
+// more of it, which rounds it to the nearest.
+__device__ __forceinline__ float left_out(float x) { return x - __uint_as_float(__float_as_uint(x) & ~0x1fffu); }
+template <class T> __device__ __forceinline__ uint32_t low_part(float x) { return __float_as_uint(left_out(x)) + (sizeof(T) == 4 ? 0x1000u : 0u); }
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-// d += a b with eleven bits of each factor, or (fp32 gradients) with the next eleven as well.  A step's column is its own, the others of
-// the product are times zero: a state that is no number, or infinite, makes dB and dC of all eight steps of its tile no numbers.
-// bh: the rounded factor.
-template <bool kFine>
-__device__ __forceinline__ void product(float (&d)[4], const float (&a)[4], const uint32_t (&bh)[2], const float (&b)[2]) {
-  uint32_t ah[4];
+// d += a b, 22 bits of each factor: a's two parts after one another, b's in columns of their own.  A step has two of the eight columns, the
+// others of its product are times zero: a state that is no number, or infinite, makes dB and dC of the four steps that share the
+// columns no numbers.  Eleven bits of each would leave dB and dC 1e-3 off in all (bf16, 16 x 331 steps of 2048 channels; so they are
+// 3e-5 off) in 294 us for 345; high and low parts in three products without columns of their own: 361 us.  The low parts of fp32 are
+// rounded: 2.6e-7 off, unrounded 4.2e-7 (the plain formula in fp32: 1.9e-7), 370 us for 365.
+template <class T> __device__ __forceinline__ void product(float (&d)[4], const float (&a)[4], const uint32_t (&b)[2]) {
+  uint32_t high[4], low[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ah[i] = tf32(a[i]);
-  mma(d, ah, bh);
-  if constexpr (kFine) {
-    uint32_t al[4], bl[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) al[i] = tf32(a[i] - __uint_as_float(ah[i] & ~0x1fffu));
-#pragma unroll
-    for (int i = 0; i < 2; ++i) bl[i] = tf32(b[i] - __uint_as_float(bh[i] & ~0x1fffu));
-    mma(d, ah, bl);
-    mma(d, al, bh);
+  for (int i = 0; i < 4; ++i) {
+    high[i] = __float_as_uint(a[i]);
+    low[i] = low_part<T>(a[i]);
   }
+  mma(d, high, b);
+  mma(d, low, b);
 }
 
 // A warp: eight channels and sixteen states.  Thread: channels 2 c and 2 c + 1 (c = lane % 4, the fragments' columns c and c + 4),
@@ -495,14 +494,13 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
   pdl_enter();
   constexpr int kWarps = kThreads / 32, kWide = 8 * kWarps / kBlocks, kPadded = 16 * kBlocks, kSlots = 8 * kBlocks;
   constexpr int kRow = kWide == 8 ? 8 : kWide + 8;           // four slots of eight channels fall into banks of their own
-  constexpr bool kFine = sizeof(T) == 4;
   using In = Share<kKeep, kWide, kPadded>;
   static_assert(In::kPairs == 1, "a thread finishes what it has prepared, out of registers");
   __shared__ float4 s_bc[kKeep][kSlots];                     // B of states n and n + 8, C of them
   __shared__ float4 s_dt[kKeep][kWide / 2];                  // of two channels: dt, and dt u
   __shared__ f2 s_dy[kKeep][kWide / 2];                      // dy of them
   __shared__ __align__(16) float s_part[3][kKeep][kSlots][kRow];           // C h, B dh, A a h[t - 1] dh of a thread's two states
-  __shared__ float s_narrow[kWarps / kBlocks][2][kKeep][kPadded + 4];   // dB, dC over a warp's channels
+  __shared__ float s_narrow[kWarps / kBlocks][2][kKeep][kPadded + 8];   // dB, dC over a warp's channels; written without bank conflicts
   const Block<kWide> p(s);
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, part = warp % kBlocks, group = warp / kBlocks;
   const int slot = part * 8 + lane / 4, n0 = part * 16 + lane / 4, w0 = group * 8 + lane % 4 * 2;     // state, channel in the block
@@ -615,15 +613,23 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
         h[t + 1][j] = fma2(a[t][j], h[t][j], mul2(d.y, j == 0 ? b.x : b.y));
       }
     }
-    // step lane / 4 is the column of the fragments that this lane has
-    const float2 column_dy = halves(s_dy[lane / 4][w0 / 2]);
-    const float2 column_du = halves(reinterpret_cast<const ulonglong2*>(&s_dt[lane / 4][w0 / 2])->y);
-    const float own_dy[2] = {column_dy.x, column_dy.y}, own_du[2] = {column_du.x, column_du.y};
-    const uint32_t own_dyh[2] = {tf32(column_dy.x), tf32(column_dy.y)}, own_duh[2] = {tf32(column_du.x), tf32(column_du.y)};
-    float dB[4] = {0, 0, 0, 0}, dC[4] = {0, 0, 0, 0};        // state n (n + 8), steps 2 (lane % 4) and the next
+    uint32_t own_dy[2], own_du[2];       // of the step whose column this lane has: columns 0 to 3 high parts, 4 to 7 low parts of these
+    float dB[4], dC[4];                  // state n (n + 8), columns 2 (lane % 4) and the next
     dA[0] = dA[1] = 0;
 #pragma unroll
     for (int t = kKeep - 1; t >= 0; --t) {
+      if (t % kHalf == kHalf - 1) {
+        const int own = t / kHalf * kHalf + lane / 4 % kHalf;
+        const float2 y2 = halves(s_dy[own][w0 / 2]), u2 = halves(reinterpret_cast<const ulonglong2*>(&s_dt[own][w0 / 2])->y);
+        const float y[2] = {y2.x, y2.y}, u[2] = {u2.x, u2.y};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          own_dy[i] = lane < 16 ? __float_as_uint(y[i]) : low_part<T>(y[i]);
+          own_du[i] = lane < 16 ? __float_as_uint(u[i]) : low_part<T>(u[i]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) dB[q] = dC[q] = 0.0f;
+      }
       const float4 bc = s_bc[t][slot];
       const f2 d = *reinterpret_cast<const f2*>(&s_dt[t][w0 / 2]), y2 = s_dy[t][w0 / 2];
       f2 dh[2], da[2];
@@ -637,20 +643,22 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
       *reinterpret_cast<f2*>(&s_part[0][t][slot][w0]) = fma2(h[t + 1][1], bc.w, mul2(h[t + 1][0], bc.z));
       *reinterpret_cast<f2*>(&s_part[1][t][slot][w0]) = fma2(dh[1], bc.y, mul2(dh[0], bc.x));
       *reinterpret_cast<f2*>(&s_part[2][t][slot][w0]) = fma2(da[1], A[1], mul2(da[0], A[0]));
-      const bool column = lane / 4 == t;
-      float by[2], bu[2];
-      uint32_t byh[2], buh[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        byh[i] = column ? own_dyh[i] : 0u;
-        buh[i] = column ? own_duh[i] : 0u;
-        by[i] = column ? own_dy[i] : 0.0f;          // fp32 gradients alone read them
-        bu[i] = column ? own_du[i] : 0.0f;
-      }
+      const bool column = lane / 4 % kHalf == t % kHalf;
+      const uint32_t by[2] = {column ? own_dy[0] : 0u, column ? own_dy[1] : 0u}, bu[2] = {column ? own_du[0] : 0u, column ? own_du[1] : 0u};
       const float2 h0 = halves(h[t + 1][0]), h1 = halves(h[t + 1][1]), d0 = halves(dh[0]), d1 = halves(dh[1]);
       const float ha[4] = {h0.x, h1.x, h0.y, h1.y}, da4[4] = {d0.x, d1.x, d0.y, d1.y};
-      product<kFine>(dC, ha, byh, by);
-      product<kFine>(dB, da4, buh, bu);
+      product<T>(dC, ha, by);
+      product<T>(dB, da4, bu);
+      if (t % kHalf == 0) {
+        // columns j and j + 4 belong together, in the lanes c and c + 2: each of the two goes on with one state
+        const bool second = lane % 4 >= 2;
+        const int n = n0 + (second ? 8 : 0), to = t + 2 * (lane % 2);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          s_narrow[group][0][to + q][n] = (second ? dB[2 + q] : dB[q]) + __shfl_xor_sync(0xffffffffu, second ? dB[q] : dB[2 + q], 2);
+          s_narrow[group][1][to + q][n] = (second ? dC[2 + q] : dC[q]) + __shfl_xor_sync(0xffffffffu, second ? dC[q] : dC[2 + q], 2);
+        }
+      }
     }
     // into the running sum with its rounding errors beside it: a sequence has thousands of terms
 #pragma unroll
@@ -663,11 +671,6 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
         dA_low[j][i] = (t - dA_sum[j][i]) - y;
         dA_sum[j][i] = t;
       }
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      s_narrow[group][0][2 * (lane % 4) + q % 2][n0 + q / 2 * 8] = dB[q];
-      s_narrow[group][1][2 * (lane % 4) + q % 2][n0 + q / 2 * 8] = dC[q];
     }
     __syncthreads();
 #pragma unroll
