@@ -462,9 +462,12 @@ struct Grads {
 };
 
 // The matrix instruction reads the upper eleven bits of a factor and leaves out the others: what that is, and (fp32 gradients) half a step
-// more of it, which rounds it to the nearest.
+// more of it, which rounds it to the nearest.  What is no number stays none: its bits may be all set, and a carry out of them is zero.
 __device__ __forceinline__ float left_out(float x) { return x - __uint_as_float(__float_as_uint(x) & ~0x1fffu); }
-template <class T> __device__ __forceinline__ uint32_t low_part(float x) { return __float_as_uint(left_out(x)) + (sizeof(T) == 4 ? 0x1000u : 0u); }
+template <class T> __device__ __forceinline__ uint32_t low_part(float x) {
+  const int bits = __float_as_int(left_out(x));
+  return (uint32_t)(sizeof(T) == 4 ? min(bits, 0x7fffefff) + 0x1000 : bits);
+}
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -474,7 +477,7 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], const
 // others of its product are times zero: a state that is no number, or infinite, makes dB and dC of the four steps that share the
 // columns no numbers.  Eleven bits of each would leave dB and dC 1e-3 off in all (bf16, 16 x 331 steps of 2048 channels; so they are
 // 3e-5 off) in 294 us for 345; high and low parts in three products without columns of their own: 361 us.  The low parts of fp32 are
-// rounded: 2.6e-7 off, unrounded 4.2e-7 (the plain formula in fp32: 1.9e-7), 370 us for 365.
+// rounded: 2.6e-7 off, unrounded 4.2e-7 (the plain formula in fp32: 1.9e-7), 383 us for 365.
 template <class T> __device__ __forceinline__ void product(float (&d)[4], const float (&a)[4], const uint32_t (&b)[2]) {
   uint32_t high[4], low[4];
 #pragma unroll
