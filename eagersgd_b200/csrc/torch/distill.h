@@ -76,6 +76,7 @@ Tensor distillation_loss(const Tensor& logits, const Tensor& values, const Tenso
     check_operand(op, "the labels", *labels, logits, at::kLong);
   }
   TORCH_CHECK(hard_weight == 0 || labels.has_value(), op, ": a hard weight without labels");
+  refuse_tangents(op, logits, values);
   check_gpu(op, logits);
   if (!differentiable(logits)) return DistillFn::run(logits, values, classes, value_of(labels), temperature, hard_weight, nullptr);
   check_capture(op, {&logits});

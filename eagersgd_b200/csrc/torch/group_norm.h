@@ -33,6 +33,15 @@ void check_float(const char* op, const char* name, const Tensor& t) {
   TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, op, ": ", name, " is ", t.scalar_type(),
               ", neither bfloat16 nor float32");
 }
+// A forward-mode derivative, which none of these operators makes: without it the result would read as a derivative of zero.
+void refuse_tangent(const char* op, const Tensor& t) {
+  TORCH_CHECK(!t.defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), op,
+              ": no forward-mode derivative goes through it");
+}
+void refuse_tangent(const char* op, const c10::optional<Tensor>& t) {
+  if (t.has_value()) refuse_tangent(op, *t);
+}
+template <class... T> void refuse_tangents(const char* op, const T&... tensors) { (refuse_tangent(op, tensors), ...); }
 // The last check: what came before it needs no GPU.
 void check_gpu(const char* op, const Tensor& t) { TORCH_CHECK(t.is_cuda(), op, ": the input is on ", t.device(), ", not on a GPU"); }
 
@@ -145,6 +154,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const Tensor& gamma, cons
     TORCH_CHECK(res->sizes() == x.sizes(), "group_norm_act: the residual ", res->sizes(), " is not of the input's size ", x.sizes());
     check_operand("group_norm_act", "the residual", *res, x, x.scalar_type());
   }
+  refuse_tangents("group_norm_act", x, gamma, beta, res);
   check_gpu("group_norm_act", x);
   const Tensor residual = value_of(res);
   if (!differentiable(x) && !differentiable(gamma) && !differentiable(beta) && !differentiable(residual))

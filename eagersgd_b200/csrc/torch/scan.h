@@ -129,6 +129,7 @@ variable_list causal_conv(const Tensor& x, const Tensor& weight, const Opt& bias
   check_lengths(op, lengths, x);
   check_state(op, state, x, {x.size(0), weight.size(1) - 1, x.size(2)}, x.scalar_type());
   TORCH_CHECK(x.size(0) * ((x.size(1) + 31) / 32) * ((x.size(2) + 31) / 32) < ((int64_t)1 << 30), op, ": an input of ", x.sizes(), " is too large");
+  refuse_tangents(op, x, weight, bias_in, state);
   check_gpu(op, x);
   const Tensor bias = value_of(bias_in);
   if (!differentiable(x) && !differentiable(weight) && !differentiable(bias))
@@ -151,6 +152,7 @@ std::pair<Tensor, Tensor> causal_conv_step(const Tensor& x_in, const Tensor& sta
   TORCH_CHECK(!differentiable(x_in) && !differentiable(weight) && !(bias.has_value() && differentiable(*bias)), op,
               ": no gradient goes through a step; call it under torch.no_grad()");
   const Tensor next = state_for(op, out, state);
+  refuse_tangents(op, x_in, state, weight, bias);
   check_gpu(op, x_in);
   c10::cuda::CUDAGuard guard(x_in.device());
   const Tensor x = rows_dense(x_in);
@@ -284,6 +286,7 @@ variable_list selective_scan(const Tensor& u, const Tensor& delta, const Tensor&
   check_scan_operands(op, u, delta, A, B, C, D_in, z, bias_in);
   check_lengths(op, lengths, u);
   check_state(op, state, u, {u.size(0), u.size(2), A.size(1)}, at::kFloat);
+  refuse_tangents(op, u, delta, A, B, C, D_in, z, bias_in, state);
   check_gpu(op, u);
   const Tensor D = value_of(D_in), bias = value_of(bias_in), gate = value_of(z);
   if (!differentiable(u) && !differentiable(delta) && !differentiable(A) && !differentiable(B) && !differentiable(C) && !differentiable(D) &&
@@ -312,6 +315,7 @@ std::pair<Tensor, Tensor> selective_scan_step(const Tensor& u, const Tensor& del
   for (const Opt* t : {&D, &z, &bias})
     TORCH_CHECK(!t->has_value() || !differentiable(**t), op, ": no gradient goes through a step; call it under torch.no_grad()");
   const Tensor next = state_for(op, out, state);
+  refuse_tangents(op, u, delta, A, B, C, state, D, z, bias);
   check_gpu(op, u);
   c10::cuda::CUDAGuard guard(u.device());
   const ScanInputs in = {rows_dense(u), rows_dense(delta), z.has_value() ? rows_dense(*z) : Tensor(), rows_dense(B), rows_dense(C), A,
