@@ -50,7 +50,7 @@ struct DistillFn : public Function<DistillFn> {
     const int64_t n = (grad.size(0) - 1) * grad.stride(0) + grad.size(1);
     ck(esgd_distill_scale(ptr(grad), mut(out), grad.scalar_type() == at::kBFloat16, fptr(factor), n, stream_of(grad)),
        "distillation_loss backward");
-    return {out, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return once("distillation_loss", grads, {out, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 

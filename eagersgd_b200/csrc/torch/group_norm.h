@@ -1,6 +1,7 @@
 // Group norm (+ residual) (+ activation) as an autograd operator; part of ops.cpp.
 #pragma once
 #include <ATen/cuda/EmptyTensor.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 extern "C" {
 int esgd_group_norm_max_group();
@@ -83,6 +84,22 @@ struct ParamGrad {
   }
 };
 
+// The gradients of a backward pass that is to be differentiated itself (create_graph): they can be used, and refuse to be differentiated.
+// As they come out of the kernels they would read as constants.  The refusal lies on the way to whatever the operator was made of, and
+// to the gradients that arrived.
+variable_list once(const char* op, const variable_list& arrived, variable_list&& grads) {
+  if (!at::GradMode::is_enabled()) return std::move(grads);
+  torch::autograd::edge_list edges = torch::autograd::collect_next_edges(arrived);
+  if (const auto node = torch::autograd::get_current_node()) edges.insert(edges.end(), node->next_edges().begin(), node->next_edges().end());
+  const auto error = std::make_shared<torch::autograd::Error>(c10::str(op, ": there is no second derivative"), std::move(edges));
+  for (Tensor& g : grads) {
+    if (!g.defined()) continue;
+    g = g.detach();
+    torch::autograd::impl::set_gradient_edge(g, {error, error->add_input_metadata(g)});
+  }
+  return std::move(grads);
+}
+
 struct GroupNormFn : public Function<GroupNormFn> {
   using Opt = c10::optional<Tensor>;
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Opt& gamma_in, const Opt& beta_in, const Opt& res_in, int64_t groups,
@@ -132,7 +149,7 @@ struct GroupNormFn : public Function<GroupNormFn> {
     dbeta.done();
     variable_list out(12);
     out[0] = dx; out[1] = dgamma.grad; out[2] = dbeta.grad; out[3] = dres;
-    return out;
+    return once("group_norm_act", grads, std::move(out));
   }
 };
 

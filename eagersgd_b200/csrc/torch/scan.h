@@ -105,7 +105,7 @@ struct CausalConvFn : public Function<CausalConvFn> {
     dw.done();
     db.done();
     out[0] = dx; out[1] = dw.grad; out[2] = db.grad;
-    return out;
+    return once("causal_conv", grads, std::move(out));
   }
 };
 
@@ -250,7 +250,7 @@ struct SelectiveScanFn : public Function<SelectiveScanFn> {
     dD.done();
     db.done();
     out[0] = du; out[1] = ddelta; out[2] = dA.grad; out[3] = dB; out[4] = dC; out[5] = dD.grad; out[6] = dz; out[7] = db.grad;
-    return out;
+    return once("selective_scan", grads, std::move(out));
   }
 };
 
