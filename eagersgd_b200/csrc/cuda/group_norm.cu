@@ -527,9 +527,12 @@ bool plan(int64_t samples, int64_t rows, int channels, int groups, int v, int si
     s->split *= 2;
   const int64_t held = v > 1 ? budget / row : 0, most = (rows + s->split - 1) / s->split;
   s->held = (int)(held < most ? held : most);
-  s->passing = samples * rows * channels * size > kPassing;
+  s->passing = (double)samples * (double)rows * channels * size > (double)kPassing;
   return true;
 }
+// CTAs of a pass; as many as a grid takes.
+int64_t ctas(const Shape& s, int64_t samples) { return samples * (s.channels / s.slice) * s.split; }
+constexpr int64_t kMostCtas = ((int64_t)1 << 31) - 1;
 
 template <int kCluster, class... K, class... A>
 int launch_cluster(void (*kernel)(K...), int64_t units, size_t smem, void* stream, A... args) {
@@ -555,6 +558,13 @@ size_t fit(Shape* s, size_t row, size_t fixed) {
   return s->held * row + fixed;
 }
 constexpr int kForwardHeld = 45 * 1024, kBackwardHeld = 64 * 1024;
+// The plan of a direction with vectors of v elements, or single ones where a slice of whole vectors is too wide.
+bool plan_of(bool backward, int64_t samples, int64_t rows, int channels, int groups, int* v, int size, Shape* s) {
+  const int tensors = backward ? 2 : 1, budget = backward ? kBackwardHeld : kForwardHeld;
+  if (plan(samples, rows, channels, groups, *v, size, tensors, budget, s)) return true;
+  *v = 1;
+  return plan(samples, rows, channels, groups, *v, size, tensors, budget, s);
+}
 
 template <class T, int kV, int kAct, bool kAdd>
 int forward(const void* x, const void* residual, void* z, const float* gamma, const float* beta, float* stats, int64_t samples,
@@ -589,6 +599,18 @@ extern "C" {
 // Channels of a group at most: a slice holds a group, kMaxSlice channels.
 int esgd_group_norm_max_group() { return kMaxSlice; }
 
+// Whether grids hold so many samples, in both directions and however the tensors lie.
+int esgd_group_norm_fits(int64_t samples, int64_t rows, int channels, int groups, int is_bf16) {
+  if (samples > kMostCtas) return 0;
+  for (int backward = 0; backward < 2; ++backward)
+    for (int most : {1, is_bf16 ? 8 : 4}) {
+      int v = channels % most ? 1 : most;
+      Shape s;
+      if (!plan_of(backward, samples, rows, channels, groups, &v, is_bf16 ? 2 : 4, &s) || ctas(s, samples) > kMostCtas) return 0;
+    }
+  return 1;
+}
+
 // x, residual, z [samples][rows][channels]; stats [samples][groups][2] (mean, 1 / deviation), or null.
 int esgd_group_norm_fwd(const void* x, const void* residual, void* z, const float* gamma, const float* beta, float* stats, int is_bf16,
                         int64_t samples, int64_t rows, int channels, int groups, int act, float eps, void* stream) {
@@ -596,10 +618,7 @@ int esgd_group_norm_fwd(const void* x, const void* residual, void* z, const floa
   int v = is_bf16 ? 8 : 4;
   if (channels % v || !aligned16(x) || !aligned16(z) || !aligned16(residual)) v = 1;
   Shape s;
-  if (!plan(samples, rows, channels, groups, v, is_bf16 ? 2 : 4, 1, kForwardHeld, &s)) {
-    v = 1;
-    if (!plan(samples, rows, channels, groups, v, is_bf16 ? 2 : 4, 1, kForwardHeld, &s)) return (int)cudaErrorInvalidValue;
-  }
+  if (!plan_of(false, samples, rows, channels, groups, &v, is_bf16 ? 2 : 4, &s) || ctas(s, samples) > kMostCtas) return (int)cudaErrorInvalidValue;
   s.eps = eps;
   return ESGD_TYPE(forward, x, residual, z, gamma, beta, stats, samples, s, stream);
 }
@@ -612,10 +631,7 @@ int esgd_group_norm_bwd(const void* x, const void* residual, const void* dz, voi
   int v = is_bf16 ? 8 : 4;
   if (channels % v || !aligned16(x) || !aligned16(residual) || !aligned16(dz) || !aligned16(dx) || !aligned16(dres)) v = 1;
   Shape s;
-  if (!plan(samples, rows, channels, groups, v, is_bf16 ? 2 : 4, 2, kBackwardHeld, &s)) {
-    v = 1;
-    if (!plan(samples, rows, channels, groups, v, is_bf16 ? 2 : 4, 2, kBackwardHeld, &s)) return (int)cudaErrorInvalidValue;
-  }
+  if (!plan_of(true, samples, rows, channels, groups, &v, is_bf16 ? 2 : 4, &s) || ctas(s, samples) > kMostCtas) return (int)cudaErrorInvalidValue;
   s.eps = 0.0f;
   return ESGD_TYPE(backward, x, residual, dz, dx, dres, gamma, beta, stats, sums, samples, s, stream);
 }

@@ -5,6 +5,7 @@
 
 extern "C" {
 int esgd_group_norm_max_group();
+int esgd_group_norm_fits(int64_t samples, int64_t rows, int channels, int groups, int is_bf16);
 int esgd_group_norm_fwd(const void* x, const void* residual, void* z, const float* gamma, const float* beta, float* stats, int is_bf16,
                         int64_t samples, int64_t rows, int channels, int groups, int act, float eps, void* stream);
 int esgd_group_norm_bwd(const void* x, const void* residual, const void* dz, void* dx, void* dres, const float* gamma, const float* beta,
@@ -163,7 +164,10 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const Tensor& gamma, cons
   TORCH_CHECK(c / groups <= esgd_group_norm_max_group(), "group_norm_act: takes up to ", esgd_group_norm_max_group(), " channels a group, not ",
               c / groups);
   TORCH_CHECK(act >= 0 && act <= 2 && eps >= 0, "group_norm_act: no such activation, or an eps below zero");
-  TORCH_CHECK(c < ((int64_t)1 << 31) && x.size(0) * c < ((int64_t)1 << 27) && x.size(2) * x.size(3) < ((int64_t)1 << 30),
+  // what the grids hold; of fewer channels in all there are not so many CTAs
+  TORCH_CHECK(c < ((int64_t)1 << 31) && x.size(2) * x.size(3) < ((int64_t)1 << 30) &&
+                  (x.size(0) <= ((int64_t)1 << 27) / c ||
+                   esgd_group_norm_fits(x.size(0), x.size(2) * x.size(3), (int)c, (int)groups, x.scalar_type() == at::kBFloat16)),
               "group_norm_act: an input of ", x.sizes(), " is too large");
   check_vector("group_norm_act", "gamma", gamma, x, c);
   check_vector("group_norm_act", "beta", beta, x, c);
