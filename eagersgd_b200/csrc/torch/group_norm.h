@@ -101,6 +101,9 @@ variable_list once(const char* op, const variable_list& arrived, variable_list&&
   return std::move(grads);
 }
 
+// Floats of room for the samples' shares of dgamma and dbeta: 64 MB, which L2 holds between the kernels that write and read them.
+constexpr int64_t kShares = 16 << 20;
+
 struct GroupNormFn : public Function<GroupNormFn> {
   using Opt = c10::optional<Tensor>;
   static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Opt& gamma_in, const Opt& beta_in, const Opt& res_in, int64_t groups,
@@ -140,12 +143,19 @@ struct GroupNormFn : public Function<GroupNormFn> {
     if (need & 8) dres = act == 0 ? dz : fresh_image(x);
     const ParamGrad dgamma(ctx, "g", need & 2, {c}, x), dbeta(ctx, "b", need & 4, {c}, x);
     void* st = stream_of(x);
-    const int64_t parts = rows > 0 ? n : 0;
-    const Tensor sums = fresh_floats({parts, 2, c}, x);
-    ck(esgd_group_norm_bwd(ptr(x), ptr(res), ptr(dz), mut(dx), act == 0 ? nullptr : mut(dres), fptr(gamma), fptr(beta), fptr(stats), fptr(sums),
-                           x.scalar_type() == at::kBFloat16, n, rows, (int)c, (int)groups, (int)act, st), "group_norm_act backward");
-    ck(esgd_sum_parts(fptr(sums), parts, dbeta.out(), c, dbeta.add(), dgamma.out(), c, dgamma.add(), nullptr, 0, 0, st),
-       "group_norm_act parameter gradients");
+    // Every sample has its share of dgamma and dbeta.  Where those of all would take more room than kShares -- samples of few pixels, whose
+    // shares are larger than they are -- the samples are worked on a portion at a time, and the gradients added up in their order.
+    const int64_t all = rows > 0 ? n : 0, portion = std::max<int64_t>(1, std::min(all, kShares / (2 * c)));
+    const Tensor sums = fresh_floats({std::min(all, portion), 2, c}, x);
+    for (int64_t first = 0; first == 0 || first < all; first += portion) {
+      const int64_t parts = std::min(portion, all - first), at = first * rows * c * x.element_size();
+      auto from = [at](const Tensor& t) -> void* { return t.defined() ? (char*)t.data_ptr() + at : nullptr; };
+      ck(esgd_group_norm_bwd(from(x), from(res), from(dz), from(dx), act == 0 ? nullptr : from(dres), fptr(gamma), fptr(beta),
+                             fptr(stats) + first * groups * 2, fptr(sums), x.scalar_type() == at::kBFloat16, parts, rows, (int)c, (int)groups,
+                             (int)act, st), "group_norm_act backward");
+      ck(esgd_sum_parts(fptr(sums), parts, dbeta.out(), c, dbeta.add() || first > 0, dgamma.out(), c, dgamma.add() || first > 0, nullptr, 0, 0,
+                        st), "group_norm_act parameter gradients");
+    }
     dgamma.done();
     dbeta.done();
     variable_list out(12);

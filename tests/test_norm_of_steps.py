@@ -73,3 +73,51 @@ def test_norms_of_steps(n, c, groups, dtype):
 @gpu
 def test_more_than_two_to_the_27_channels_in_all():
     _against_the_formula(16 * 4099, 2048, 1, BF16)
+
+
+@gpu
+@pytest.mark.parametrize("n,c,dtype", [(64000, 1024, BF16), (20000, 2048, F32)])
+def test_the_backward_pass_takes_no_more_room_than_it_leaves(n, c, dtype):
+    """... and 64 MB: a sample's share of dgamma and dbeta is four times a bf16 sample of one pixel."""
+    x, dz = _steps(n, c, dtype)
+    p = [torch.ones(c, device="cuda", requires_grad=True) for _ in range(2)]
+    z = ops.group_norm_act(x.requires_grad_(), 1, *p)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(z, [x, *p], dz)
+    torch.cuda.synchronize()
+    left = torch.cuda.memory_allocated() - before
+    assert left < x.numel() * x.element_size() + (1 << 21)
+    assert torch.cuda.max_memory_allocated() - before < left + (64 << 20) + (1 << 21)
+    del grads
+
+
+@gpu
+def test_a_portion_more_goes_where_the_first_one_went():
+    """Into an accumulator of a training step, and beside samples of an odd number and a shortcut with an activation."""
+    n, c = 9001, 2048                                                          # portions of 4096
+    x, dz = _steps(n, c, BF16)
+    gamma, beta = (torch.nn.Parameter(torch.randn(c, device="cuda")) for _ in range(2))
+    leaves = [x.requires_grad_(), gamma, beta, dz.clone().requires_grad_()]
+    f = lambda v, r: ops.group_norm_act(v, 4, gamma, beta, "silu", r)  # noqa: E731
+    dx, dgamma, dbeta, dres = torch.autograd.grad(f(x, leaves[3]), leaves, dz)
+    want = [torch.zeros(c, device="cuda") for _ in range(2)]
+    for i in range(0, n, 4096):
+        v, r, d = (t.detach()[i:i + 4096] for t in (x, leaves[3], dz))
+        part = torch.autograd.grad(f(v.requires_grad_(), r.requires_grad_()), [v, gamma, beta, r], d)
+        assert torch.equal(part[0], dx[i:i + 4096]) and torch.equal(part[3], dres[i:i + 4096])
+        want[0] += part[1]
+        want[1] += part[2]
+    assert torch.equal(dgamma, want[0]) and torch.equal(dbeta, want[1])
+    sinks = _build.load_torch().GradSinks([2], lambda bucket: None)
+    acc = [torch.full((c,), 0.5, device="cuda") for _ in range(2)]
+    for p, a in zip((gamma, beta), acc):
+        sinks.add(p, a, 0)
+    sinks.begin_step()
+    sinks.set_active(True)
+    f(x, leaves[3]).backward(dz)
+    sinks.set_active(False)
+    sinks.close()
+    for a, w in zip(acc, want):
+        near(a, w.double() + 0.5, w.double().abs() + 0.5, 8, "accumulator")
