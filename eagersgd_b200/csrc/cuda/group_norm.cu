@@ -169,8 +169,13 @@ template <class T, int kV, int kMany> struct Rows {
   __device__ __forceinline__ Pack<T, kV> first(const Place<kV>& pl, int v) const {
     return load<T, kV>(kV > 1 && pl.lane < held ? in + pl.lane * slice + v * kV : p[0] + pl.lane * pitch + v * kV);
   }
-  // use(vectors, the vector of `more`, their offset from p[]) for a thread's rows; kAhead of them are loaded at a time.
+  // use(vectors, the vector of `more`, their offset from p[]) for a thread's rows; kAhead of them are loaded at a time, and then used()
+  // is called (behind single rows it is not: those are fewer than kAhead, twice).
   template <int kAhead, bool kMore, class Use> __device__ __forceinline__ void each(const Place<kV>& pl, int v, const T* more, Use use) const {
+    each<kAhead, kMore>(pl, v, more, use, [] {});
+  }
+  template <int kAhead, bool kMore, class Use, class Used>
+  __device__ __forceinline__ void each(const Place<kV>& pl, int v, const T* more, Use use, Used used) const {
     const int lanes = pl.lanes, n = kV == 1 ? 0 : held < pl.rows ? held : pl.rows, next = lanes * slice;
     const int64_t down = lanes * pitch;
     const T* own = in + pl.lane * slice + v * kV;
@@ -186,6 +191,7 @@ template <class T, int kV, int kMany> struct Rows {
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) use(x[u], e[u], o + u * down);
+      used();
     }
     for (; r < n; r += lanes, o += down, own += next) {
       if constexpr (kMore) e[0] = load<T, kV>(more + o);
@@ -202,6 +208,7 @@ template <class T, int kV, int kMany> struct Rows {
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) use(x[u], e[u], o + u * down);
+      used();
     }
     for (; r < pl.rows; r += lanes, o += down) {
       if constexpr (kMore) e[0] = load<T, kV>(more + o);
@@ -250,8 +257,10 @@ group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T
   in.ask<false>(p);
   arrived();
   const float inv_rows = rows > 0 ? 1.0f / (float)rows : 0.0f;
-  // a thread's rows about its first one of a channel, which is one of them: what the squares lose to it is as many roundings as it
-  // has rows at most; threads, channels and CTAs are then joined as means and squared deviations
+  // A thread's rows about a centre: its first one, and after 4, 8, 16, ... of them the mean so far.  Up to the next of these the squares
+  // about that centre are at most twice those about the mean, so that they lose no more than the roundings of a sum of so many terms.
+  // (About the first row alone, were it an outlier, they would be as many times as large as there are rows: 1e-3 of the variance with
+  // 1024 of them.)  Threads, channels and CTAs are then joined as means and squared deviations.
   const float own_rows = (float)(rows > p.lane ? (rows - p.lane + p.lanes - 1) / p.lanes : 0), inv_own = own_rows > 0.0f ? 1.0f / own_rows : 0.0f;
   for (int v0 = 0; v0 < p.vectors; v0 += p.wide) {
     const int v = v0 + p.vec;
@@ -260,7 +269,9 @@ group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T
       unpack2<T, kV>(in.first(p, v), first);
 #pragma unroll
       for (int q = 0; q < kP; ++q) first[q] = mul2(first[q], -1.0f);
+      int seen = 0, next = 4;
       in.template each<4, false>(p, v, nullptr, [&](const Pack<T, kV>(&raw)[1], const Pack<T, kV>&, int64_t) {
+        ++seen;
         f2 f[kP];
         unpack2<T, kV>(raw[0], f);
 #pragma unroll
@@ -268,6 +279,17 @@ group_norm_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, T
           const f2 d = add2(f[q], first[q]);
           a[0][q] = add2(a[0][q], d);
           square[q] = fma2(d, d, square[q]);
+        }
+      }, [&] {
+        if (seen < next) return;
+        next = 2 * seen;
+        const float n = (float)seen, inv = 1.0f / n;
+#pragma unroll
+        for (int q = 0; q < kP; ++q) {
+          const f2 to = fma2(a[0][q], -inv, first[q]), by = add2(first[q], mul2(to, -1.0f));       // -centre, and how far that moved
+          square[q] = fma2(mul2(by, -1.0f), fma2(by, -n, mul2(a[0][q], 2.0f)), square[q]);
+          a[0][q] = fma2(by, -n, a[0][q]);
+          first[q] = to;
         }
       });
     }
