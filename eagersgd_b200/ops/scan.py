@@ -85,9 +85,11 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
         r = _build.load_torch().selective_scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, return_state)
         return tuple(r) if return_state else r[0]
     uw, dw, Aw, Bw, Cw, Dw, zw, bw = _wide(u, delta, A, B, C, D, z, delta_bias)
+    inside = _inside(u.shape[1], lengths, u)
+    if lengths is not None:         # a value behind the end meets nothing: times the zero of a gradient it could still be no number
+        uw, dw, Bw, Cw, zw = (None if v is None else torch.where(inside.unsqueeze(2), v, 0.0) for v in (uw, dw, Bw, Cw, zw))
     dt = dw if bw is None else dw + bw
     dt = F.softplus(dt) if softplus else dt
-    inside = _inside(u.shape[1], lengths, u)
     h = uw.new_zeros(u.shape[0], *A.shape) if state is None else state.detach().to(uw.dtype)
     outs = []
     for t in range(u.shape[1]):
