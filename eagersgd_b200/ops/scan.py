@@ -38,6 +38,15 @@ def _inside(length: int, lengths: Optional[torch.Tensor], like: torch.Tensor) ->
     return (t < lengths.unsqueeze(1)) if lengths is not None else torch.ones(like.shape[0], length, dtype=torch.bool, device=like.device)
 
 
+def _one_step(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Sequences of no step with a step of zeros."""
+    return None if x is None else F.pad(x, (0, 0, 0, 1))
+
+
+def _no_step(x: torch.Tensor) -> torch.Tensor:
+    return torch.zeros(x.shape[0], dtype=torch.int64, device=x.device)
+
+
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = "silu",
                 state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
                 return_state: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
@@ -50,6 +59,9 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         r = _build.load_torch().causal_conv(x, weight, bias, act, state, lengths, return_state)
         return tuple(r) if return_state else r[0]
     taps, length = weight.shape[1], x.shape[1]
+    if length == 0:                 # as one step that none of the sequences has
+        y, last = causal_conv(_one_step(x), weight, bias, activation, state, _no_step(x), True)
+        return (y[:, :0], last) if return_state else y[:, :0]
     xw, w, b = _wide(x, weight, bias)
     inside = _inside(length, lengths, x)
     ahead = xw.new_zeros(x.shape[0], taps - 1, x.shape[2]) if state is None else state.detach().to(xw.dtype)
@@ -84,6 +96,9 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     if native_float(u):
         r = _build.load_torch().selective_scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, return_state)
         return tuple(r) if return_state else r[0]
+    if u.shape[1] == 0:
+        y, h = selective_scan(*map(_one_step, (u, delta)), A, *map(_one_step, (B, C)), D, _one_step(z), delta_bias, softplus, state, _no_step(u), True)
+        return (y[:, :0], h) if return_state else y[:, :0]
     uw, dw, Aw, Bw, Cw, Dw, zw, bw = _wide(u, delta, A, B, C, D, z, delta_bias)
     inside = _inside(u.shape[1], lengths, u)
     if lengths is not None:         # a value behind the end meets nothing: times the zero of a gradient it could still be no number
@@ -100,7 +115,7 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
         y = y if Dw is None else y + Dw * uw[:, t]
         y = y if zw is None else y * F.silu(zw[:, t])
         outs.append(torch.where(live.squeeze(2), y, 0.0))
-    y = (torch.stack(outs, 1) if outs else torch.zeros_like(uw)).to(u.dtype)
+    y = torch.stack(outs, 1).to(u.dtype)
     return (y, h.detach()) if return_state else y
 
 

@@ -38,3 +38,24 @@ def test_what_lies_behind_a_sequence_is_nobodys(dtype, spoil, softplus):
         results.append((y.detach(), last, *torch.autograd.grad(y, leaves, dy)))
     for a, b in zip(*results):
         assert torch.isfinite(b).all() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("b,t", [(0, 5), (3, 0), (0, 0)])
+@pytest.mark.parametrize("dtype", [F32, F64])
+def test_empty_sequences_and_batches(b, t, dtype):
+    c, dy, state = _scan_case(b, t, 6, 4, dtype, "cpu")
+    leaves = {k: v.detach().requires_grad_() for k, v in c.items()}
+    y, h = scan.selective_scan(**leaves, state=state, return_state=True)
+    assert y.shape == (b, t, 6) and y.dtype == dtype and torch.equal(h, state.to(h.dtype))
+    for g, k in zip(torch.autograd.grad(y, list(leaves.values()), dy), leaves):
+        assert g.shape == leaves[k].shape and not g.any()
+    assert scan.selective_scan(**dict(c, D=None, z=None, delta_bias=None)).shape == (b, t, 6)
+    for k in (2, 4):
+        x, w, bias, dy = _conv_case(b, t, 6, k, dtype, "cpu")
+        leaves = [v.requires_grad_() for v in (x, w, bias)]
+        ahead = torch.randn(b, k - 1, 6, dtype=dtype)
+        y, last = scan.causal_conv(*leaves, state=ahead, return_state=True)
+        assert y.shape == (b, t, 6) and torch.equal(last, ahead)
+        for g, v in zip(torch.autograd.grad(y, leaves, dy), leaves):
+            assert g.shape == v.shape and not g.any()
+        assert scan.causal_conv(x, w).shape == (b, t, 6)
