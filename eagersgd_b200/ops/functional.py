@@ -253,16 +253,19 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     wide = logits if logits.dtype == torch.float64 else logits.float()
     classes, t = logits.shape[1], temperature
     named = (teacher_classes >= 0) & (teacher_classes < classes) & (teacher_logits != -float("inf"))
+    if hard_weight == 1:            # nobody is taught
+        named = torch.zeros_like(named)
     values = torch.where(named, teacher_logits.detach().to(wide.dtype) / t, -float("inf"))
     taught = named.any(1, keepdim=True)
     log_p = torch.log_softmax(torch.where(taught, values, 0.0), 1)
-    log_q = torch.log_softmax(wide / t, 1).gather(1, teacher_classes.clamp(0, classes - 1))
+    # a row that has no such term: zero times the derivative of whatever its logits are could be no number
+    log_q = torch.log_softmax(torch.where(taught, wide, 0.0) / t, 1).gather(1, teacher_classes.clamp(0, classes - 1))
     p = torch.where(named, log_p.exp(), 0.0)
     kl = torch.where(p != 0, p * (torch.where(p != 0, log_p, 0.0) - torch.where(p != 0, log_q, 0.0)), 0.0).sum(1)
     loss = (1.0 - hard_weight) * t * t * kl.sum() / logits.shape[0]
     if hard_weight != 0:
         valid = (labels >= 0) & (labels < classes)
-        ce = F.cross_entropy(wide, torch.where(valid, labels, 0), reduction="none")
+        ce = F.cross_entropy(torch.where(valid.unsqueeze(1), wide, 0.0), torch.where(valid, labels, 0), reduction="none")
         loss = loss + hard_weight * torch.where(valid, ce, 0.0).sum() / logits.shape[0]
     return loss
 
