@@ -17,7 +17,7 @@ struct DistillFn : public Function<DistillFn> {
     Tensor grad;
     Tensor loss = run(logits, values.t, classes.t, labels.t, temperature, hard_weight, &grad);
     ctx->save_for_backward({grad});
-    ctx->saved_data["captured"] = capturing(logits);
+    ctx->saved_data["capture"] = capture_of(logits);
     return loss;
   }
   // grad: also the gradient for a factor of one, rows as far apart as those of the logits where these are the dense layer's padded
@@ -38,14 +38,14 @@ struct DistillFn : public Function<DistillFn> {
     return loss;
   }
   // The gradient is there; times the factor that arrives.  Where this is its only use it is scaled where it lies, and the kernel
-  // returns at once for a factor of one (loss.backward()); a graph that is kept, and one whose backward pass alone is captured and
-  // would scale the buffer once a replay, gets a product of its own.  Another factor rounds a
-  // bf16 gradient a second time: the price of not reading the logits again.
+  // returns at once for a factor of one (loss.backward()).  A graph that is kept gets a product of its own, and so does one whose
+  // backward pass is captured without its forward pass, or apart from it: every replay of that alone would scale the buffer once
+  // more.  Another factor rounds a bf16 gradient a second time: the price of not reading the logits again.
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const Tensor grad = ctx->get_saved_variables()[0];
     c10::cuda::CUDAGuard guard(grad.device());
     const Tensor factor = grads[0].to(at::kFloat).contiguous();
-    const bool kept = torch::autograd::get_current_graph_task_keep_graph() || (!ctx->saved_data["captured"].toBool() && capturing(grad));
+    const bool kept = torch::autograd::get_current_graph_task_keep_graph() || ctx->saved_data["capture"].toInt() != capture_of(grad);
     Tensor out = kept ? at::empty_strided(grad.sizes(), grad.strides(), grad.options()) : grad;
     const int64_t n = (grad.size(0) - 1) * grad.stride(0) + grad.size(1);
     ck(esgd_distill_scale(ptr(grad), mut(out), grad.scalar_type() == at::kBFloat16, fptr(factor), n, stream_of(grad)),

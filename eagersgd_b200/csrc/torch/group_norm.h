@@ -52,6 +52,13 @@ bool capturing(const Tensor& t) {
   return cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream(t.get_device()).stream(), &status) == cudaSuccess &&
          status != cudaStreamCaptureStatusNone;
 }
+// The capture that the current stream is part of, 0: none.
+int64_t capture_of(const Tensor& t) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  return cudaStreamGetCaptureInfo(c10::cuda::getCurrentCUDAStream(t.get_device()).stream(), &status, &id) == cudaSuccess &&
+         status != cudaStreamCaptureStatusNone ? (int64_t)id : 0;
+}
 
 // A gradient that goes to `t` ends in the node that adds it to t.grad, on the stream that node was made on.  In a capture that has
 // to be the capturing stream: a node left by an eager graph that is still alive is on another one, and the engine's waiting for it
