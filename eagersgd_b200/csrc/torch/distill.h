@@ -68,8 +68,10 @@ Tensor distillation_loss(const Tensor& logits, const Tensor& values, const Tenso
               classes.sizes(), " classes for ", logits.size(0), " rows");
   TORCH_CHECK(values.size(1) <= esgd_distill_max_top(), op, ": takes up to ", esgd_distill_max_top(), " of a teacher's logits, not ", values.size(1));
   TORCH_CHECK(logits.size(0) <= ((int64_t)1 << 27) && logits.size(1) < ((int64_t)1 << 31) - 8, op, ": logits of ", logits.sizes(), " are too many");
-  TORCH_CHECK(std::isfinite(temperature) && temperature > 0 && hard_weight >= 0 && hard_weight <= 1, op, ": a temperature of ", temperature,
-              " and a hard weight of ", hard_weight);
+  // the kernel has T, 1 / T and T^2 in fp32
+  const float t = (float)temperature;
+  TORCH_CHECK(t > 0 && std::isnormal(t * t) && hard_weight >= 0 && hard_weight <= 1, op, ": a temperature of ",
+              temperature, " and a hard weight of ", hard_weight);
   TORCH_CHECK(!values.requires_grad() || !at::GradMode::is_enabled(), op, ": the teacher's logits get no gradient: detach them");
   if (labels.has_value()) {
     TORCH_CHECK(labels->numel() == logits.size(0), op, ": ", labels->numel(), " labels for ", logits.size(0), " rows");

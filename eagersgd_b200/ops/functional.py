@@ -250,6 +250,8 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         return _ext().distillation_loss(logits, teacher_logits, teacher_classes, temperature, labels, hard_weight)
     if labels is None and hard_weight != 0:
         raise ValueError("distillation_loss: a hard weight without labels")
+    if not (0 < temperature < float("inf") and 0 <= hard_weight <= 1):
+        raise ValueError("distillation_loss: a temperature of %r and a hard weight of %r" % (temperature, hard_weight))
     wide = logits if logits.dtype == torch.float64 else logits.float()
     classes, t = logits.shape[1], temperature
     named = (teacher_classes >= 0) & (teacher_classes < classes) & (teacher_logits != -float("inf"))
