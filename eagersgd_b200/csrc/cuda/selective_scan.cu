@@ -192,6 +192,17 @@ template <int kLanes> struct Lanes : Share<kTile, 2 * kThreads / kLanes, kLanes 
   static constexpr int kRow = 2 * kThreads / kLanes + (32 / kLanes - 2 * kThreads / kLanes % 32 + 32) % 32;
 };
 
+// h e^(x ln 2), by way of a chunk.  In two halves, of which neither is infinite before the result is, nor zero; and a state of zero stays
+// zero, whatever the chunk would have made of another.
+__device__ __forceinline__ float across(float h, float x) {
+  const float half = exp2_approx(0.5f * x);
+  return h == 0.0f ? 0.0f : h * half * half;
+}
+__device__ __forceinline__ f2 across(f2 h, f2 x) {
+  const float2 v = halves(h), w = halves(x);
+  return pair(across(v.x, w.x), across(v.y, w.y));
+}
+
 // The states that a thread begins with: those given, and the other chunks' joined to them; of two channels, four states each.
 template <int kLanes, bool kReverse>
 __device__ __forceinline__ void joined(const Scan& s, int64_t b, int chunk, int channel, int two, int lane, const f2 (&a)[kStates], f2 (&h)[kStates]) {
@@ -202,7 +213,7 @@ __device__ __forceinline__ void joined(const Scan& s, int64_t b, int chunk, int 
     const float4 l = local[0], r = two > 1 ? local[kLanes] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const float own[2][4] = {{l.x, l.y, l.z, l.w}, {r.x, r.y, r.z, r.w}};
 #pragma unroll
-    for (int j = 0; j < kStates; ++j) h[j] = fma2(exp2_2(mul2(span, a[j])), h[j], pair(own[0][j], own[1][j]));
+    for (int j = 0; j < kStates; ++j) h[j] = add2(across(h[j], mul2(span, a[j])), pair(own[0][j], own[1][j]));
   }
 }
 // A value of two channels' four states each, zero where there is none.
@@ -522,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 3) selective_scan_bwd_kernel(Scan s,
       if (is && s.chunks > 1)
         for (int q = s.chunks - 1; q > p.chunk; --q) {
           const int64_t at = (q * s.batch + p.b) * s.channels + channel + i;
-          c[i] = fmaf(exp2_approx(s.span[at] * (v[i] * kLog2e)), c[i], s.local[at * g.kept + n]);
+          c[i] = across(c[i], s.span[at] * (v[i] * kLog2e)) + s.local[at * g.kept + n];
         }
     }
     A[j] = pair(v[0], v[1]);
