@@ -85,12 +85,15 @@ class ScanLayer(nn.Module):
 
 
 class ScanClassifier(nn.Module):
-    """Stacked scan layers over per-frame feature vectors, linear head on the last step; stands where ``LSTMClassifier`` does."""
+    """Stacked scan layers over per-frame feature vectors, linear head on the last step; stands where ``LSTMClassifier`` does.
+    ``dropout``: between the layers, in training, as there."""
+
+    dropout = 0.0                            # also of networks that were saved without it
 
     def __init__(self, input_dim: int = 2048, hidden: int = 1024, layers: int = 2, num_classes: int = 101, width: Optional[int] = None,
-                 states: int = 16, taps: int = 4):
+                 states: int = 16, taps: int = 4, dropout: float = 0.0):
         super().__init__()
-        self.hidden = hidden
+        self.hidden, self.dropout = hidden, dropout
         self.w_embed = nn.Parameter(torch.empty(hidden, input_dim).uniform_(-1, 1) / math.sqrt(input_dim))
         self.layers = nn.ModuleList(ScanLayer(hidden, width or 2 * hidden, states, taps) for _ in range(layers))
         self.fc = nn.Linear(hidden, num_classes)
@@ -106,12 +109,15 @@ class ScanClassifier(nn.Module):
         b, t = x.shape[:2]
         h = _project(x.reshape(b * t, -1), self.w_embed).unflatten(0, (b, t))
         states = []
-        for layer in self.layers:
-            h = layer(h, lengths, return_state)
+        for i, layer in enumerate(self.layers):
+            h = layer(self._between(i, h), lengths, return_state)
             if return_state:
                 h, s = h
                 states.append(s)
         return h, states
+
+    def _between(self, i, h):
+        return nn.functional.dropout(h, self.dropout) if i > 0 and self.dropout > 0 and self.training else h
 
     def hidden_states(self, x, lengths=None):
         """x [B, T, input_dim] -> the top layer's outputs [T, B, hidden]."""
@@ -136,6 +142,6 @@ class ScanClassifier(nn.Module):
     def step(self, x, state: State) -> torch.Tensor:
         """Logits after one step more, x [B, input_dim]; ``state`` is moved on in place."""
         h = _project(x, self.w_embed)
-        for layer, s in zip(self.layers, state):
-            h = layer.step(h, s)
+        for i, (layer, s) in enumerate(zip(self.layers, state)):
+            h = layer.step(self._between(i, h), s)
         return ops.linear(h, self.fc.weight, self.fc.bias)

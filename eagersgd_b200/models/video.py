@@ -34,7 +34,7 @@ class ResNetLSTM(nn.Module):
         self.feature_dim, self.frame_chunk = feature_dim, frame_chunk
         # the LSTM stack of the sequence classifier, with a head applied at every time step instead of the last
         self.rnn = LSTMClassifier(feature_dim, hidden, layers, num_classes, dropout=dropout) if sequence == "lstm" else \
-            ScanClassifier(feature_dim, hidden, layers, num_classes)
+            ScanClassifier(feature_dim, hidden, layers, num_classes, dropout=dropout)
 
     def compute_dtype_(self, dtype):
         self.rnn.compute_dtype_(dtype)
