@@ -62,7 +62,7 @@ class ScanLayer(nn.Module):
     def forward(self, h, lengths=None, return_state=False):
         """h [B, T, hidden] -> the same, and the layer's state behind the last step of every sequence."""
         b, t = h.shape[:2]
-        rows = lambda v: v.reshape(b * t, -1)  # noqa: E731
+        rows = lambda v: v.flatten(0, 1)  # noqa: E731
         steps = lambda v: v.unflatten(0, (b, t))  # noqa: E731
         xz = steps(self._ahead(rows(h)))
         conv = scan.causal_conv(xz[..., :self.width], self.conv_weight, self.conv_bias, lengths=lengths, return_state=return_state)
@@ -107,7 +107,7 @@ class ScanClassifier(nn.Module):
 
     def _stack(self, x, lengths=None, return_state=False):
         b, t = x.shape[:2]
-        h = _project(x.reshape(b * t, -1), self.w_embed).unflatten(0, (b, t))
+        h = _project(x.flatten(0, 1), self.w_embed).unflatten(0, (b, t))
         states = []
         for i, layer in enumerate(self.layers):
             h = layer(self._between(i, h), lengths, return_state)
