@@ -15,6 +15,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from .. import _build
 
@@ -175,6 +176,12 @@ def native_float(x: torch.Tensor) -> bool:
     return x.is_cuda and x.dtype in (torch.bfloat16, torch.float32) and not _reference_only
 
 
+def refuse_derivative(op: str, what: str, t: Optional[torch.Tensor]) -> None:
+    """What the kernels make no derivative of has none in the plain forms: left out without a word it would read as zero."""
+    if t is not None and (t.requires_grad and torch.is_grad_enabled() or forward_ad.unpack_dual(t).tangent is not None):
+        raise RuntimeError("%s: no gradient goes through %s: detach it" % (op, what))
+
+
 def group_norm_act(x: torch.Tensor, groups: int, gamma: torch.Tensor, beta: torch.Tensor, activation: Optional[str] = None,
                    residual: Optional[torch.Tensor] = None, eps: float = BN_EPS) -> torch.Tensor:
     """z = act(gamma * (x - mean) / sqrt(var + eps) + beta [+ residual]) with the statistics of a sample's group of channels.
@@ -252,12 +259,13 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         raise ValueError("distillation_loss: a hard weight without labels")
     if not (0 < temperature < float("inf") and 0 <= hard_weight <= 1):
         raise ValueError("distillation_loss: a temperature of %r and a hard weight of %r" % (temperature, hard_weight))
+    refuse_derivative("distillation_loss", "the teacher's logits", teacher_logits)
     wide = logits if logits.dtype == torch.float64 else logits.float()
     classes, t = logits.shape[1], temperature
     named = (teacher_classes >= 0) & (teacher_classes < classes) & (teacher_logits != -float("inf"))
     if hard_weight == 1:            # nobody is taught
         named = torch.zeros_like(named)
-    values = torch.where(named, teacher_logits.detach().to(wide.dtype) / t, -float("inf"))
+    values = torch.where(named, teacher_logits.to(wide.dtype) / t, -float("inf"))
     taught = named.any(1, keepdim=True)
     log_p = torch.log_softmax(torch.where(taught, values, 0.0), 1)
     # a row that has no such term: zero times the derivative of whatever its logits are could be no number

@@ -22,7 +22,7 @@ import torch
 import torch.nn.functional as F
 
 from .. import _build
-from .functional import activation_code, native_float
+from .functional import activation_code, native_float, refuse_derivative
 
 _TAKEN = (None, "silu")
 
@@ -58,6 +58,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if native_float(x):
         r = _build.load_torch().causal_conv(x, weight, bias, act, state, lengths, return_state)
         return tuple(r) if return_state else r[0]
+    refuse_derivative("causal_conv", "a state", state)
     taps, length = weight.shape[1], x.shape[1]
     if length == 0:                 # as one step that none of the sequences has
         y, last = causal_conv(_one_step(x), weight, bias, activation, state, _no_step(x), True)
@@ -96,6 +97,7 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     if native_float(u):
         r = _build.load_torch().selective_scan(u, delta, A, B, C, D, z, delta_bias, softplus, state, lengths, return_state)
         return tuple(r) if return_state else r[0]
+    refuse_derivative("selective_scan", "a state", state)
     if u.shape[1] == 0:
         y, h = selective_scan(*map(_one_step, (u, delta)), A, *map(_one_step, (B, C)), D, _one_step(z), delta_bias, softplus, state, _no_step(u), True)
         return (y[:, :0], h) if return_state else y[:, :0]
