@@ -47,6 +47,7 @@ Tensor state_for(const char* op, const Opt& out, const Tensor& state) {
   if (!out.has_value()) return at::empty_like(state);
   TORCH_CHECK(out->sizes() == state.sizes() && out->is_contiguous(), op, ": out ", out->sizes(), " is no room for a state of ", state.sizes());
   check_operand(op, "out", *out, state, state.scalar_type());
+  TORCH_CHECK(!differentiable(*out), op, ": no gradient goes through out: detach it");
   const char *a = (const char*)state.data_ptr(), *b = (const char*)out->data_ptr();
   TORCH_CHECK(a == b || a + state.nbytes() <= b || b + out->nbytes() <= a, op, ": out overlaps the state without being it");
   return *out;

@@ -3,10 +3,11 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
+from eagersgd_b200 import _build
 from eagersgd_b200.ops import functional as ops
 from eagersgd_b200.ops import scan
 from test_distillation import _case
-from test_scan import _conv_case, _scan_case
+from test_scan import CONV_STEP_FITS, STEP_FITS, _conv_case, _scan_case
 
 F64 = torch.float64
 
@@ -38,3 +39,12 @@ def test_refused(name):
         with pytest.raises(RuntimeError, match="detach it"):
             f(fwd.make_dual(t, torch.ones_like(t)))
     assert torch.equal(f(t.clone().requires_grad_().detach()), want)
+
+
+@pytest.mark.parametrize("op,fits", [("causal_conv_step", CONV_STEP_FITS), ("selective_scan_step", STEP_FITS)])
+def test_room_for_a_state_that_wants_a_gradient(op, fits):
+    f, room = getattr(_build.load_torch(), op), torch.zeros_like(fits["state"])
+    with pytest.raises(RuntimeError, match="detach it"):
+        f(*dict(fits, out=room.requires_grad_()).values())
+    with torch.no_grad(), pytest.raises(RuntimeError, match="not on a GPU"):
+        f(*dict(fits, out=room).values())
