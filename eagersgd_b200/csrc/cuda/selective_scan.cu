@@ -1005,8 +1005,9 @@ int esgd_selective_scan_bwd(const esgd_scan* e, const void* dout, const float* k
 
 int esgd_selective_scan_step(const esgd_scan* e, float* state_out, void* out, void* stream) {
   const Scan s = scan_of(e, false);
-  if (!taken(s) || s.state == nullptr) return (int)cudaErrorInvalidValue;
+  if (!taken(s)) return (int)cudaErrorInvalidValue;
   if (s.batch == 0) return 0;
+  if (s.state == nullptr) return (int)cudaErrorInvalidValue;
   const int is_bf16 = e->is_bf16, lanes = lanes_of(s.states);
   return ESGD_TYPE(step, s, state_out, out, stream);
 }
