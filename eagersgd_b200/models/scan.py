@@ -22,6 +22,8 @@ State = List[Tuple[torch.Tensor, torch.Tensor]]
 
 def _project(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """[rows, in] -> [rows, out] in x's type."""
+    if x.shape[0] == 0:                      # the kernels refuse a product of no row
+        return nn.functional.linear(x, w)
     return ops.conv1x1(x.reshape(x.shape[0], x.shape[1], 1, 1), w.reshape(*w.shape, 1, 1)).reshape(x.shape[0], w.shape[0])
 
 
@@ -128,15 +130,20 @@ class ScanClassifier(nn.Module):
             return h[:, -1]
         return h[torch.arange(h.shape[0], device=h.device), lengths.clamp(1, h.shape[1]) - 1]
 
+    def _logits(self, h):
+        if h.shape[0] == 0:
+            return nn.functional.linear(h, self.fc.weight, self.fc.bias).to(torch.float32 if ops.native(h) else h.dtype)
+        return ops.linear(h, self.fc.weight, self.fc.bias)
+
     def forward(self, x, lengths=None):
         """x [B, T, input_dim] -> logits [B, classes] of every sequence's last step."""
-        return ops.linear(self._last(self._stack(x, lengths)[0], lengths).contiguous(), self.fc.weight, self.fc.bias)
+        return self._logits(self._last(self._stack(x, lengths)[0], lengths).contiguous())
 
     @torch.no_grad()
     def prompt(self, x, lengths=None) -> Tuple[torch.Tensor, State]:
         """Logits as ``forward`` gives them, and the state that ``step`` goes on from."""
         h, states = self._stack(x, lengths, True)
-        return ops.linear(self._last(h, lengths).contiguous(), self.fc.weight, self.fc.bias), states
+        return self._logits(self._last(h, lengths).contiguous()), states
 
     @torch.no_grad()
     def step(self, x, state: State) -> torch.Tensor:
@@ -144,4 +151,4 @@ class ScanClassifier(nn.Module):
         h = _project(x, self.w_embed)
         for i, (layer, s) in enumerate(zip(self.layers, state)):
             h = layer.step(self._between(i, h), s)
-        return ops.linear(h, self.fc.weight, self.fc.bias)
+        return self._logits(h)
