@@ -5,8 +5,8 @@
 //   dz_j     = ((1 - w) T (q_j - sum_{k: i_k = j} p_k) + w (r_j - [j = label])) / rows
 //
 // Bound by memory and, nearly as much, by the exponentials: a row is read from memory once (running maxima and sums), is found in L2
-// the second time, and its gradient is written once.  (4096 x 32000 bf16, top 64: 119 us, 4.4 TB/s of 6.5; rows held in registers in
-// between, 64 KB a block and a third of the warps: 154 us.)  A block has a row, or a cluster of blocks has one where rows are fewer
+// the second time, and its gradient is written once.  (4096 x 32000 bf16, top 64: 121 us, 4.4 TB/s of 6.5; rows held in registers in
+// between, 64 KB a block and a third of the warps: 119 -> 154 us.)  A block has a row, or a cluster of blocks has one where rows are fewer
 // than SMs; their maxima and sums meet in distributed shared memory.  The few classes that the teacher or the label names are
 // written again, from their own sums, after the others: a class that is named twice counts twice.  An index outside the classes is
 // no class; a row without a teacher (or label) has no such term, whatever its logits are.

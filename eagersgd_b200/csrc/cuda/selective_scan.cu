@@ -26,12 +26,12 @@
 // registers from the first half of a tile to the second, and four blocks an SM: 1061 us for 1035; arithmetic without pairs: 1125 for
 // 1072.)
 //
-// The exponentials are those of the special function units, of dt A log2 e as fp32 rounds it: a state's decay is off by some 2e-7.  That
-// shows in dA alone, 4.6e-7 off in fp32 (3 x 77 steps of 500 channels) where exponentials right to half a step leave 2.4e-7.  Putting
-// the argument's rounding right is no help (4.6e-7, and 143 us for 90 forward at 16 x 331 x 2048): the units' own error remains.
+// The exponentials are those of the special function units, of dt A log2 e as fp32 rounds it, some 2e-7 off.  dA of fp32 sequences is 4.6e-7
+// off in all (3 x 77 steps of 500 channels; the plain formula in fp32: 2.4e-7).  Putting the argument's rounding right left that as it was
+// and took 143 us for 90 forward (16 x 331 x 2048).
 //
 // Kept for the backward pass are 4 bytes a state, every eighth step: 8 bytes a step and channel with 16 states (16 with 17 to 32, and so on by
-// powers of two), four times a bf16 u.  That pass has shares of dB and dC, 256 bytes a step and 32 channels of up to 16 states.
+// powers of two), four times a bf16 u.  That pass has shares of dB and dC, 128 bytes a step and 32 channels of up to 16 states.
 //
 // Few sequences of few channels: the steps are split into chunks that run at the same time.  A first pass scans every chunk from a
 // state of zero; what a chunk begins with is then the chunks ahead of it joined, h = exp(A sum dt) h + (its own scan).
