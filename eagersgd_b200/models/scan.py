@@ -109,7 +109,7 @@ class ScanClassifier(nn.Module):
 
     def _stack(self, x, lengths=None, return_state=False):
         b, t = x.shape[:2]
-        h = _project(x.flatten(0, 1), self.w_embed).unflatten(0, (b, t))
+        h = _project(x.flatten(0, 1).flatten(1), self.w_embed).unflatten(0, (b, t))
         states = []
         for i, layer in enumerate(self.layers):
             h = layer(self._between(i, h), lengths, return_state)

@@ -33,3 +33,9 @@ def test_no_sequence_on_the_gpu():
 def test_no_step_has_no_last_one():
     with pytest.raises(IndexError):
         ScanClassifier(8, 16, 2, 5)(torch.randn(2, 0, 8))
+
+
+def test_frames_of_more_dimensions_are_laid_flat():
+    net = ScanClassifier(24, 16, 1, 5)
+    x = torch.randn(2, 6, 2, 3, 4)
+    assert torch.equal(net(x), net(x.reshape(2, 6, 24)))
