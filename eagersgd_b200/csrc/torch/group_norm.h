@@ -166,8 +166,11 @@ struct GroupNormFn : public Function<GroupNormFn> {
     dgamma.done();
     dbeta.done();
     variable_list out(12);
-    out[0] = dx; out[1] = dgamma.grad; out[2] = dbeta.grad; out[3] = dres;
-    return once("group_norm_act", grads, std::move(out));
+    out[0] = dx; out[1] = dgamma.grad; out[2] = dbeta.grad;
+    if (act != 0) out[3] = dres;
+    out = once("group_norm_act", grads, std::move(out));
+    if (act == 0) out[3] = dres;         // what arrived, with a derivative of its own
+    return out;
   }
 };
 

@@ -14,7 +14,7 @@ def _calls(dev="cuda", dtype=torch.float32):
     image, p, seq, narrow, taps = r(2, 8, 3, 3), r(8), r(2, 7, 6), r(2, 7, 4), r(6, 3)
     values, named = r(2, 3), torch.tensor([[1, 2, 3], [4, 5, 6]], device=dev)
     return {"group_norm_act": (image, lambda x: ops.group_norm_act(x, 2, p, p, "silu")),
-            "group_norm_act, shortcut": (image, lambda x: ops.group_norm_act(image.detach(), 2, p, p, None, x)),
+            "group_norm_act, shortcut": (image, lambda x: ops.group_norm_act(image.detach(), 2, p, p, "silu", x)),
             "distillation_loss": (r(2, 9), lambda x: ops.distillation_loss(x, values, named)),
             "causal_conv": (seq, lambda x: scan.causal_conv(x, taps)),
             "selective_scan": (seq, lambda x: scan.selective_scan(x, seq, -torch.ones(6, 4, dtype=dtype, device=dev), narrow, narrow))}
@@ -34,6 +34,17 @@ def test_refused_once_it_is_asked_for(name):
         torch.autograd.grad((first * x).sum(), x, retain_graph=True)
     with pytest.raises(RuntimeError, match="no second derivative"):
         (first * x).sum().backward()
+
+
+@gpu
+def test_a_shortcut_without_activation_has_them_all():
+    """Its gradient is the one that arrives."""
+    x, p = torch.randn(2, 8, 3, 3, device="cuda", requires_grad=True), torch.ones(8, device="cuda")
+    image = torch.randn(2, 8, 3, 3, device="cuda")
+    z = ops.group_norm_act(image, 2, p, p, None, x)
+    first, = torch.autograd.grad((z ** 3).sum(), x, create_graph=True)
+    second, = torch.autograd.grad((first * image).sum(), x)
+    assert torch.allclose(second, 6 * z.detach() * image, rtol=1e-5, atol=1e-5)
 
 
 @gpu
