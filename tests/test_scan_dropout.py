@@ -51,3 +51,20 @@ def test_a_network_saved_without_it_has_none():
     del net.__dict__["dropout"]
     x = torch.randn(3, 6, 8)
     assert torch.equal(net(x), net(x))
+
+
+@pytest.mark.gpu
+def test_in_a_captured_training_step():
+    """Every replay drops others: the losses of one batch at a rate of zero differ."""
+    from eagersgd_b200.ops import functional as ops
+    from eagersgd_b200.parallel.group import Group
+    from eagersgd_b200.train.step import TrainStep
+    torch.manual_seed(0)
+    x, y = torch.randn(8, 17, 64, device="cuda").to(torch.bfloat16), torch.arange(8, device="cuda")
+    for dropout in (0.0, 0.5):
+        step = TrainStep(ScanClassifier(64, 96, 2, 40, width=160, dropout=dropout), Group(), mode="solo", limiter=4, lr=0.0, momentum=0.0,
+                         weight_decay=0.0, loss_fn=ops.softmax_cross_entropy)
+        step.capture(x, y)
+        losses = [float(step.run_device(x, y)) for _ in range(4)]
+        assert all(v == v for v in losses) and len(set(losses)) == (4 if dropout else 1)
+        step.close()
